@@ -69,7 +69,7 @@ static __device__ __forceinline__ void abx3_for(F&& f) {
 // 3 RoPE state, 4 both folds done, 5 fragments in AGPRs, 6 first W image, 7 first block landed, 8.. start of every block, then
 // drain start, end.  PREFOLD: 0 start, 1 low fragments requested, 2 they have landed and the table values are in registers (barriers
 // A, A2), 3 high fragments and first block requested + RoPE state, 4 = 3, 5 first W image, 6 high fragments landed (barrier B), 7 fragments in AGPRs (barrier
-// C) + second block requested, 8.. blocks.  The stamps use scalar registers only: the TIMING build does not spill.
+// C) + second block requested, 8.. blocks.
 // PREFOLD (round 6): the folded fragments come from p.qfold (abx_fold.h: written once per launch by the projection kernel's q
 // waves or by abx_fold_kernel) instead of being folded from (p.a, p.bfrag2) by every workgroup.  The prologue is then: the
 // RoPE start tables (3 loads per wave, shared through LDS) + the folded LOW fragments by LDS-DMA -> wait, barrier -> table
@@ -100,15 +100,15 @@ __global__ __launch_bounds__(ABX3_THREADS) __attribute__((amdgpu_waves_per_eu(1,
   const int hi = lane >> 5;
   const int g = blockIdx.x % p.G;
   const int cidx = blockIdx.x / p.G;
-  // (TIMING: scalar registers only -- s_memtime into an SGPR pair, s_store_dwordx2 through the scalar cache, written back at
-  //  the kernel's end: the R = 128 kernel has no VGPR to spare, round 5's vector-store stamps made the TIMING build spill)
+  // (TIMING: s_memtime into an SGPR pair, lane 0 stores it.  The R = 128 kernel has no VGPR to spare: this store makes the
+  //  TIMING build spill a little, so its stamps are an upper bound)
   unsigned stamp_off = 0;
   unsigned long long* const dbg_w = TIMING ? p.dbg + ((size_t)blockIdx.x * 4 + w) * 64 : nullptr;
   auto stamp = [&]() {
     if constexpr (TIMING) {
       unsigned long long t;                         // (no branch: stamps past the 64th wrap around inside the wave's own row)
       asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)" : "=s"(t));
-      asm volatile("s_store_dwordx2 %0, %1, %2" ::"s"(t), "s"(dbg_w), "s"(stamp_off) : "memory");
+      if (lane == 0) dbg_w[stamp_off >> 3] = t;
       stamp_off = (stamp_off + 8) & (64 * 8 - 1);
     }
   };
@@ -903,7 +903,6 @@ __global__ __launch_bounds__(ABX3_THREADS) __attribute__((amdgpu_waves_per_eu(1,
   finalize(b - 1);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the re-read pieces of the last blocks: nothing may land in LDS after the wave ends)
   stamp();
-  if constexpr (TIMING) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb" ::: "memory");
 #undef ABX3_MFMA_A0
 #undef ABX3_MFMA_A
 #undef ABX3_MFMA_V0

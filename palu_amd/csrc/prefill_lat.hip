@@ -126,11 +126,11 @@ __global__ __launch_bounds__(PL_THREADS, 1) void prefill_lat_kernel(PfLatParams 
   unsigned stamp_off = 0;
   unsigned long long* const dbg_w = p.dbg + w * 64;
   const bool stamp_on = p.dbg != nullptr && blockIdx.x == 0 && blockIdx.y == 0;
-  auto stamp = [&](int jt) {                          // scalar registers only (abx_rope3_kernel.h)
+  auto stamp = [&](int jt) {
     if (stamp_on && jt >= 16 && jt < 24) {
       unsigned long long t;
       asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)" : "=s"(t));
-      asm volatile("s_store_dwordx2 %0, %1, %2" ::"s"(t), "s"(dbg_w), "s"(stamp_off) : "memory");
+      if ((threadIdx.x & 63) == 0) dbg_w[stamp_off >> 3] = t;
       stamp_off = (stamp_off + 8) & (64 * 8 - 1);
     }
   };
@@ -738,9 +738,6 @@ __global__ __launch_bounds__(PL_THREADS, 1) void prefill_lat_kernel(PfLatParams 
         }
     }
   }
-#ifdef PL_TIMELINE
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb" ::: "memory");
-#endif
 }
 
 // cos / sin of the key positions as the reference's rotary cache holds them (kernel/palu_attention.py:204: rotary_emb; HF
