@@ -15,7 +15,9 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libpalu_hip.so")
-CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc"]
+# (-packed-fp32-ops: some forms of the packed fp32 instructions that hipcc makes from ordinary float code have given wrong results on this
+# hardware now and then; scalar forms give the same values)
+CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file flags: the position-split score kernel schedules its VALU work by hand (no packed fp32 forms)
 FILE_FLAGS = {"abx_rope3.hip": ["-fno-slp-vectorize", "-Rpass-analysis=kernel-resource-usage"]}
 # kernels that must not touch scratch: the position-split score kernel sits at 256 VGPRs + 256 AGPRs with hand-placed
