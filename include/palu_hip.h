@@ -488,6 +488,46 @@ int palu_exchange_allreduce_f32(const void* src, size_t bytes, const void* peers
                                 size_t slot_bytes, void* out, palu_stream_t stream);
 int palu_exchange_status(const void* buffer, unsigned* epoch_host, unsigned* error_host);
 
+/* ------------------------------------------------------------------------------------------
+ * Pages of a 4-bit latent cache that many sequences share (the reference decodes one sequence over one contiguous cache:
+ * kernel/palu_attention.py:207-257; its fake-quantised rows: palu/model/modules/quant.py:29-41).
+ *
+ *   k_codes [layers][N][G][P][Rk / 2] bytes   k_meta [layers][N][G][P][2] fp16 = (scale, zero)   (v_* alike with Rv)
+ *
+ * contiguous, 16-byte aligned; a row's codes and pair are those of palu_quantize_pack with bits = 4.  A page holds P
+ * consecutive positions (P a power of two >= 16) of one sequence; row b of block_table (row stride st_b elements, max_pages
+ * entries) lists the pages of sequence b in order.  Entries past a sequence's last row are never read.  Ranks are multiples of 8.
+ *
+ * palu_paged_append_q4: quantises row t of k [T][G][Rk] / v [T][G][Rv] (element strides, rows 16-byte aligned) and writes it as
+ * position positions[t] of sequence seq_ids[t].  A negative id or position marks a padding row, which is skipped, and so is a row
+ * whose sequence, table entry or page does not exist.  Two rows of one call must not name the same place.
+ *
+ * palu_paged_copy: page dst[i] becomes a copy of page src[i] for all i < n, in every layer.  The targets must be distinct and none
+ * of them a source; a pair that names a page outside 0 .. N - 1 is skipped.
+ *
+ * palu_paged_attn_q4: one token of each of B sequences: with x, v the de-quantised latents ((code - zero) * scale, unrounded),
+ *   ctx[b, h] = sum_l softmax_l(sm_scale <q, R(l) (x_l B_h)>) v_l          l < seq_lens[b], fp32 accumulation, fp16 out
+ * q [B][H][128] fp16 (strides sq_b, sq_h).  q_positions NULL: q is rotated already; else it is not, and q_positions[b] is its
+ * position (the rotation is applied inside).  bfrag: palu_paged_prepare_b's layout of B [H][Rk][128] (made once, a weight).
+ * ctx [B][H][Rv] contiguous.  A sequence of length 0 gives zeros; a length beyond max_pages * P or a page outside the pool within
+ * the length gives NaN for that sequence (nothing outside the pool is read).  Rk <= 256, Rv <= 512.
+ * The workspace may be reused once the call's work is done; two calls that run at the same time need one each.
+ */
+int palu_paged_append_q4(const void* k, int64_t sk_t, int64_t sk_g, const void* v, int64_t sv_t, int64_t sv_g,
+                         void* k_codes, void* k_meta, void* v_codes, void* v_meta,
+                         const int* block_table, int64_t st_b, int B, int max_pages, const int* seq_ids, const int* positions,
+                         int T, int G, int P, int n_pages, int Rk, int Rv, palu_stream_t stream);
+int palu_paged_copy(void* k_codes, void* k_meta, void* v_codes, void* v_meta, const int* src, const int* dst, int n,
+                    int layers, int n_pages, int G, int P, int Rk, int Rv, palu_stream_t stream);
+size_t palu_paged_b_bytes(int H, int G, int Rk);
+int palu_paged_prepare_b(const void* b, int H, int G, int Rk, int D, void* bfrag, palu_stream_t stream);
+size_t palu_paged_attn_workspace_bytes(int B, int H, int G, int max_pages, int P, int Rk, int Rv);
+int palu_paged_attn_q4(const void* q, int64_t sq_b, int64_t sq_h, const void* bfrag,
+                       const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta,
+                       const int* block_table, int64_t st_b, int max_pages, const int* seq_lens, const int* q_positions,
+                       const float* inv_freq, void* ctx, void* workspace, int B, int H, int G, int D, int P, int n_pages,
+                       int Rk, int Rv, float sm_scale, palu_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

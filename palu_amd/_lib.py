@@ -113,6 +113,14 @@ SIGNATURES = {
     "palu_pack_codes": (i32, [vp, vp, i64, i32, vp]),
     "palu_unpack_codes": (i32, [vp, vp, i64, i32, vp]),
     "palu_hadamard_transform": (i32, [vp, vp, i64, i32, f32, i32, vp]),
+    "palu_paged_append_q4": (i32, [vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, i32, i32, i32,
+                                   i32, vp]),
+    "palu_paged_copy": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp]),
+    "palu_paged_b_bytes": (sz, [i32, i32, i32]),
+    "palu_paged_prepare_b": (i32, [vp, i32, i32, i32, i32, vp, vp]),
+    "palu_paged_attn_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, i32]),
+    "palu_paged_attn_q4": (i32, [vp, i64, i64, vp, vp, vp, vp, vp, vp, i64, i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32,
+                                 i32, i32, f32, vp]),
     "palu_exchange_bytes": (sz, [i32, sz]),
     "palu_exchange_alloc": (i32, [sz, C.POINTER(C.c_void_p)]),
     "palu_exchange_free": (i32, [vp]),
