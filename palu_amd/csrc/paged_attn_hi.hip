@@ -1,0 +1,7 @@
+// paged_attn_kernel (paged_attn_kernel.h) for key ranks up to 12 and 16 blocks of 16 columns; a translation unit of its own so that the
+// instances compile side by side.
+#include "paged_attn_kernel.h"
+
+int palu_paged_attn_launch_hi(const void* params, int nks, int subsets, int heads, int wgs, hipStream_t stream) {
+  return pa_launch<12, 16>(*reinterpret_cast<const PagedAttnParams*>(params), nks, subsets, heads, wgs, stream);
+}

@@ -1,0 +1,7 @@
+// paged_attn_kernel (paged_attn_kernel.h) for key ranks up to 6 and 8 blocks of 16 columns; a translation unit of its own so that the
+// instances compile side by side.
+#include "paged_attn_kernel.h"
+
+int palu_paged_attn_launch_mid(const void* params, int nks, int subsets, int heads, int wgs, hipStream_t stream) {
+  return pa_launch<6, 8>(*reinterpret_cast<const PagedAttnParams*>(params), nks, subsets, heads, wgs, stream);
+}
