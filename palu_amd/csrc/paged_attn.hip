@@ -2,9 +2,9 @@
 // of a sequence.  The attention itself is paged_attn_kernel.h.
 #include "paged_attn_kernel.h"
 
-int palu_paged_attn_launch_lo(const void* params, int nks, int subsets, int heads, int wgs, hipStream_t stream);
-int palu_paged_attn_launch_mid(const void* params, int nks, int subsets, int heads, int wgs, hipStream_t stream);
-int palu_paged_attn_launch_hi(const void* params, int nks, int subsets, int heads, int wgs, hipStream_t stream);
+int palu_paged_attn_launch_lo(const void* params, int nks, int chunks, int heads, int wgs, hipStream_t stream);
+int palu_paged_attn_launch_mid(const void* params, int nks, int chunks, int heads, int wgs, hipStream_t stream);
+int palu_paged_attn_launch_hi(const void* params, int nks, int chunks, int heads, int wgs, hipStream_t stream);
 
 namespace {
 
@@ -60,10 +60,14 @@ __global__ __launch_bounds__(256) void paged_prepare_b_kernel(const h16* __restr
   const int g = gv / VG, hl = heads * (gv - g * VG) + 2 * mb + (n >> 4);
   const int col = 8 * w + 4 * ((n >> 3) & 1) + 2 * ((n >> 2) & 1) + (e >> 1) + 64 * (e & 1);
   h16x8 v;
+  // 16-byte piece u of a position's row in LDS is word i of part `part` of the row; the last parts are moved back to end with the row,
+  // and what they then hold a second time counts for nothing
+  const int u = 2 * kb + (lane >> 5), ul = nks / 2, part = u / ul, i = u % ul;
+  const int word = min(part * ul, R / 8 - ul) + i;
 #pragma unroll
   for (int d = 0; d < 8; ++d) {
-    const int r = (2 * kb + (lane >> 5)) * 8 + (d >> 1) + 4 * (d & 1);
-    v[d] = hl < gs && r < R ? b[((int64_t)(g * gs + hl) * R + r) * 128 + col] : (h16)0.f;
+    const int r = 8 * word + (d >> 1) + 4 * (d & 1);
+    v[d] = hl < gs && word >= part * ul ? b[((int64_t)(g * gs + hl) * R + r) * 128 + col] : (h16)0.f;
   }
   out[idx] = __builtin_bit_cast(u32x4, v);
 }
@@ -80,14 +84,13 @@ int pa_heads(int H, int G, int R) { return H / G <= 2 || R > 128 ? 2 : 4; }
 int pa_vg(int H, int G, int R) { return (H / G + pa_heads(H, G, R) - 1) / pa_heads(H, G, R); }
 
 struct PaPlan {
-  int tile, wgs, slots, min_chunk, direct;
+  int wgs, slots, min_chunk, direct;
 };
 // Workgroups of a launch: what the device holds at once, at most one per min_chunk tiles of the longest possible batch.
 PaPlan pa_plan(int B, int H, int G, int max_pages, int P, int Rk) {
   PaPlan s;
   const int64_t gv = (int64_t)G * pa_vg(H, G, Rk);
-  s.tile = pa_nks(Rk) <= 8 ? PaLds<8>::TILE : PaLds<16>::TILE;
-  const int64_t tiles = ((int64_t)max_pages * P + s.tile - 1) / s.tile;       // of the longest sequence the table has room for
+  const int64_t tiles = ((int64_t)max_pages * P + PA_TILE - 1) / PA_TILE;     // of the longest sequence the table has room for
   s.min_chunk = 1;
   s.direct = tiles <= s.min_chunk;
   if (s.direct) {
@@ -153,13 +156,13 @@ extern "C" int palu_paged_attn_q4(const void* q, int64_t sq_b, int64_t sq_h, con
   const int heads = pa_heads(H, G, Rk);
   const PagedAttnParams p = {(const h16*)q, sq_b, sq_h, (const h16*)bfrag, (const unsigned*)k_codes, (const unsigned*)k_meta,
                              (const unsigned*)v_codes, (const unsigned*)v_meta, block_table, st_b, seq_lens, q_positions, inv_freq,
-                             (h16*)ctx, (float*)workspace, s.slots, B, H, G, H / G, VG, max_pages, log_p, n_pages, Rk, Rv, heads, s.tile,
+                             (h16*)ctx, (float*)workspace, s.slots, B, H, G, H / G, VG, max_pages, log_p, n_pages, Rk, Rv, heads,
                              s.min_chunk, s.direct, sm_scale * 1.44269504088896f};
-  const int subsets = Rv <= 128 ? 4 : Rv <= 256 ? 2 : 1;
+  const int chunks = (Rv + 127) / 128;
   hipStream_t st = (hipStream_t)stream;
-  const int rc = nks <= 4 ? palu_paged_attn_launch_lo(&p, nks, subsets, heads, s.wgs, st)
-                 : nks <= 8 ? palu_paged_attn_launch_mid(&p, nks, subsets, heads, s.wgs, st)
-                            : palu_paged_attn_launch_hi(&p, nks, subsets, heads, s.wgs, st);
+  const int rc = nks <= 4 ? palu_paged_attn_launch_lo(&p, nks, chunks, heads, s.wgs, st)
+                 : nks <= 8 ? palu_paged_attn_launch_mid(&p, nks, chunks, heads, s.wgs, st)
+                            : palu_paged_attn_launch_hi(&p, nks, chunks, heads, s.wgs, st);
   if (rc != PALU_OK || s.direct) return rc;
   hipLaunchKernelGGL(paged_attn_join_kernel, dim3((unsigned)(B * G * VG), (unsigned)heads, (unsigned)((Rv + 63) / 64)), dim3(256), 0, st, p,
                      s.wgs);

@@ -11,28 +11,28 @@
 //
 // Work: 2 Rk 512 + 2 Rv 4 flops a position and group of four heads against Rk / 2 + Rv / 2 + 8 bytes -- 500 flops a byte, so the
 // matrix pipe and the vector units bound it, not the memory.  Split:
-//   * A workgroup (8 waves) takes a range of tiles (128 positions; 64 where Rk > 128) of one (sequence, four heads of one latent
-//     group: two where Rk > 128, whose fragments fill the registers).  The tiles of the whole batch are one line, cut into gridDim.x equal pieces, so ragged batches need no plan from the
-//     host and replay in a graph; a piece that covers a sequence's end goes on with the next.  Pieces of one sequence are joined by
-//     a second kernel.
-//   * Scores: wave w owns the RoPE pairs 8 w .. 8 w + 7 of all heads.  Its part of F stays in registers (4 heads x 16 columns x Rk:
-//     64 VGPRs at Rk = 128) as the A operand of v_mfma_f32_32x32x16_f16, two heads an instruction; a tile's codes are turned into
-//     fp16 once, by all eight waves, and shared through LDS as the B operand.  A lane then holds 4 pairs of ONE position for two
-//     heads, and the cos / sin of those 4 pairs, advanced from block to block by a rotation (exact again every 32 tiles), serve
-//     all heads.  The eight waves' partial scores meet in LDS.
-//   * Softmax and values: wave w owns an eighth of a tile's positions, with its own running maximum and sums; the eight are joined
-//     at the end of the range.  A lane holds eight columns of one row, and v_mfma_f32_4x4x4_16b_f16 (16 independent blocks of
-//     4 heads x 4 positions x 4 columns) wastes no row on the four heads a group has.
-//   * The values of tile t - 1 run in the same barrier interval as the scores of tile t, in front of them in waves 4 .. 7 and behind
-//     them in waves 0 .. 3: the two waves of a SIMD keep the matrix pipe and the vector unit busy at the same time.
+//   * A workgroup (12 waves, three a SIMD) takes a range of 128-position tiles of one (sequence, four heads of one latent group; two
+//     where Rk > 128, whose fragments fill the registers).  The work of the whole batch is one line, cut into
+//     gridDim.x equal pieces, so ragged batches need no plan from the host and replay in a graph; a piece that covers a sequence's end
+//     goes on with the next.  Pieces of one sequence are joined by a second kernel.
+//   * Scores: eight waves, wave w owns the RoPE pairs 8 w .. 8 w + 7 of all heads.  Its part of F stays in registers (4 heads x 16
+//     columns x Rk: 64 VGPRs at Rk = 128) as the A operand of v_mfma_f32_32x32x16_f16, two heads an instruction; a tile's codes are
+//     turned into fp16 once, by all eight waves, and shared through LDS as the B operand.  A lane then holds 4 pairs of ONE position
+//     for two heads, and the cos / sin of those 4 pairs, advanced from block to block by a rotation (exact again every 32 tiles),
+//     serve all heads.  The eight waves' partial scores meet in LDS.
+//   * Softmax and values: four waves, one a SIMD, each with 32 of a tile's positions and its own running maximum and sums, joined at
+//     the end of the range; they work on tile t - 1 while the others score tile t, so that the vector work of the values runs beside
+//     the matrix chains of the scores.  A lane holds eight columns of eight rows, as loaded, and so the B operands of eight
+//     v_mfma_f32_16x16x32_f16 (32 positions, 16 columns each; the four heads' weights fill its 16 rows four times over).  Smaller
+//     blocks (4x4x4, no idle row) were slower: every matrix instruction of a value wave waits for those of two score waves.
 #pragma once
 #include "palu_common.h"
 
 namespace {
 
-constexpr int PA_THREADS = 512;
+constexpr int PA_THREADS = 768;
 constexpr int PA_FIX = 3;                // cost of starting and ending a piece, in tiles (measured: 6 us against 2 us a tile)
-constexpr int PA_SLAB = 2048;            // floats of a (wave, subset) slab times subsets: [4 heads][512 / S columns] of the epilogue
+constexpr int PA_TILE = 128;             // positions of a tile
 
 struct PagedAttnParams {
   const h16* q;       int64_t sq_b, sq_h;
@@ -49,7 +49,6 @@ struct PagedAttnParams {
   int B, H, G, gs, VG;                   // gs = H / G heads of a latent group, dealt into VG sets of `heads` (2 or 4)
   int max_pages, log_p, n_pages, Rk, Rv;
   int heads;
-  int tile;                              // positions of a tile
   int min_chunk;                         // tiles a workgroup takes at least
   int direct;                            // one workgroup per (sequence, heads): no partial results, no second kernel
   float scale;                           // sm_scale log2(e)
@@ -60,7 +59,7 @@ static __device__ __forceinline__ int pa_rows(const PagedAttnParams& p, int b) {
   return min(max(p.lens[b], 0), p.max_pages << p.log_p);
 }
 static __device__ __forceinline__ bool pa_bad_len(const PagedAttnParams& p, int b) { return p.lens[b] > (p.max_pages << p.log_p); }
-static __device__ __forceinline__ int pa_tiles(const PagedAttnParams& p, int b) { return (pa_rows(p, b) + p.tile - 1) / p.tile; }
+static __device__ __forceinline__ int pa_tiles(const PagedAttnParams& p, int b) { return (pa_rows(p, b) + PA_TILE - 1) / PA_TILE; }
 
 // The line of all work: sequences in order, for each its G VG sets of heads in order, for each a fixed part (the fold of the query and
 // the join of the waves, PA_FIX tiles' worth) and its tiles.  The line is cut into gridDim.x equal pieces.
@@ -98,11 +97,14 @@ static __device__ __forceinline__ int pa_chunk(const PagedAttnParams& p, int tot
   return max((total + W - 1) / W, p.min_chunk + PA_FIX);
 }
 
-// maximum over the 16 lanes of a DPP row
+// maximum / sum over the 16 lanes of a DPP row.  (The maximum as the DPP form of v_max itself: from fmaxf over a DPP move hipcc makes
+// five instructions a step.  A value may be read through DPP two wait states after it was written.)
 static __device__ __forceinline__ float row_max16(float v) {
-#define PA_ROR(N) v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xf, 0xf, false)))
-  PA_ROR(1); PA_ROR(2); PA_ROR(4); PA_ROR(8);
-#undef PA_ROR
+  asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:1 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:2 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:4 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 0" : "+v"(v));
   return v;
 }
 static __device__ __forceinline__ float row_sum16(float v) {
@@ -111,42 +113,73 @@ static __device__ __forceinline__ float row_sum16(float v) {
 #undef PA_ROR
   return v;
 }
+// Keeps hipcc from computing ahead of a loop what is made from v: few values are worth a register through it.
+template <class T>
+static __device__ __forceinline__ void pa_opaque(T& v) { asm volatile("" : "+v"(v)); }
+static __device__ __forceinline__ float pa_other(float v, int lane) {        // v of another lane
+  return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * lane, __builtin_bit_cast(int, v)));
+}
+// a word at a scalar address plus 32 bits of the lane's own: the form of a load that needs no vector address arithmetic
+static __device__ __forceinline__ unsigned lane_word(const unsigned* row, unsigned bytes) {
+  return *reinterpret_cast<const unsigned*>(reinterpret_cast<const char*>(row) + bytes);
+}
 static __device__ __forceinline__ float lane_value(float v, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-template <int NKS>
+// N consecutive words alike, as few wide loads (a word's alignment is enough for them)
+template <int N>
+static __device__ __forceinline__ void lane_words(unsigned* out, const unsigned* row, unsigned bytes) {
+  constexpr int V = N <= 4 ? N : N / 2;
+  typedef unsigned vec __attribute__((ext_vector_type(V)));
+  typedef vec vec4 __attribute__((aligned(4)));
+#pragma unroll
+  for (int i = 0; i < N / V; ++i) {
+    const vec v = *reinterpret_cast<const vec4*>(reinterpret_cast<const char*>(row + i * V) + bytes);
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[i * V + j] = v[j];
+  }
+}
+
+// Exponent of the largest element of head lane >> 4's query, less 4 (0 for a query of zeros, or one that is not finite).
+static __device__ __forceinline__ int pa_query_exponent(const h16* q, int64_t sq_h, int nh, int lane) {
+  const h16x8 q8 = *reinterpret_cast<const h16x8*>(q + min(lane >> 4, nh - 1) * sq_h + 8 * (lane & 15));
+  float big = 0.f;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) big = fmaxf(big, fabsf((float)q8[d]));
+  big = row_max16(big);
+  return big > 0.f && big < INFINITY ? (int)(__builtin_bit_cast(unsigned, big) >> 23) - 131 : 0;
+}
+
+template <int NKS, int NH>
 struct PaLds {
-  static constexpr int TILE = NKS <= 8 ? 128 : 64;
   static constexpr int XS = NKS * 32 + 16;                 // bytes of a position's row: 16 more, so that 8 lanes reading 16 bytes of 8 rows meet 8 bank groups
-  static constexpr int RED = 2 * TILE * XS;                // float [2][8 waves][4 heads][TILE]
-  static constexpr int WGT = RED + 2 * 8 * 4 * TILE * 4;   // h16 [8 waves]: weights [4 heads][16], zeros [16]
-  static constexpr int STEP = WGT + 8 * 80 * 2;            // f32x4 [8 waves][2 halves][2]: cos / sin of a 32-position step
+  static constexpr int RED = 2 * PA_TILE * XS;             // float [2][8 waves][NH heads][PA_TILE]
+  static constexpr int WGT = RED + 2 * 8 * NH * PA_TILE * 4;   // h16 [4 waves]: weights [4 heads][32], zeros [32]
+  static constexpr int STEP = WGT + 4 * 160 * 2;           // f32x4 [8 waves][2 halves][2]: cos / sin of a 32-position step
   static constexpr int LOOP = STEP + 8 * 64;
-  static constexpr int STAT = 8 * PA_SLAB * 4;             // (epilogue, over the loop's) float [8 waves][4 heads][4], sums [4], maxima [4]
-  static constexpr int BYTES = LOOP > STAT + 576 ? LOOP : STAT + 576;
+  static constexpr int STAT = 4 * 4 * 512 * 4;             // (epilogue, over the loop's) float slabs [4 waves][4 heads][512], then
+  static constexpr int BYTES = LOOP > STAT + 160 ? LOOP : STAT + 160;   // statistics [4 waves][4 heads][2], sums [4], maxima [4]
 };
 
-// NKS: 16-column blocks of the (padded) key rank.  S: rows of values a wave holds side by side (Rv <= 512 / S).  NH: heads computed.
-template <int NKS, int S, int NH>
-__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_kernel(PagedAttnParams p) {
-  using L = PaLds<NKS>;
-  constexpr int TILE = L::TILE;
-  constexpr int ROWS = TILE / 8;                           // positions of a tile that a wave owns
+// NKS: 16-column blocks of the (padded) key rank.  NC: 128-column chunks of the (padded) value rank.  NH: heads computed.
+template <int NKS, int NC, int NH>
+__global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnParams p) {
+  using L = PaLds<NKS, NH>;
+  constexpr int TILE = PA_TILE;
   constexpr int NB = TILE / 32;                            // 32-position blocks
   constexpr int MB = NH / 2;                               // matrix blocks of two heads
-  constexpr int KL = 64 / ROWS;                            // lanes of a key row
-  constexpr int UL = 2 * NKS / KL;                         // words of codes such a lane turns into fp16
-  constexpr int ST = ROWS / (4 * S);                       // steps of 4 positions a block takes through a wave's rows
-  static_assert(ST >= 1 && UL * KL == 2 * NKS, "a wave's rows");
+  constexpr int KROWS = TILE / 8;                          // key rows of a tile that a score wave turns into fp16
+  constexpr int KL = 64 / KROWS;                           // lanes of a key row
+  constexpr int UL = 2 * NKS / KL;                         // words of codes of such a lane
+  static_assert(UL * KL == 2 * NKS, "a row's words");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 31, hi = lane >> 5;
   const int GV = p.G * p.VG;
   float* const red = reinterpret_cast<float*>(smem + L::RED);
-  h16* const wgt = reinterpret_cast<h16*>(smem + L::WGT) + w * 80;
-  const f32x4* const step = reinterpret_cast<const f32x4*>(smem + L::STEP) + w * 4 + hi * 2;
+  float* const slab = reinterpret_cast<float*>(smem);
+  float* const stat = reinterpret_cast<float*>(smem + L::STAT);
 
   // ---- this workgroup's piece of the line
   int at = 0, end = 0;
@@ -215,154 +248,48 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_kernel(PagedAttnPara
     const int qp = p.qpos ? p.qpos[b] : 0;
     const int* const table = p.table + (int64_t)b * p.st_b;
 
-    // Pages of this wave's positions (ROWS of a tile, never across a page's end), of 64 tiles at once: lane i has tile tb + i's, so
-    // that no tile waits for the table.  None: 0 (a page that exists; the rows are masked); outside the pool: -1.
-    int pages = 0, tb = t0;
-    auto load_pages = [&]() {
-      const int64_t l = (int64_t)(tb + lane) * TILE + ROWS * w;
-      pages = 0;
+    const int log_p = p.log_p, kw = p.Rk >> 3, vw = p.Rv >> 3;
+    // Pages of 16 positions of a tile (never across a page's end), of 64 tiles at once: lane i has tile tb + i's, so that no tile waits
+    // for the table.  None: 0 (a page that exists; the rows are masked); outside the pool: -1.
+    auto load_pages = [&](int tb, int offset) {
+      const int64_t l = (int64_t)(tb + lane) * TILE + offset;
+      int pg = 0;
       if (tb + lane < t1 && l < rows) {
-        pages = table[l >> p.log_p];
-        if (pages >= p.n_pages) pages = -1;
+        pg = table[l >> log_p];
+        if (pg >= p.n_pages) pg = -1;
       }
+      return pg;
     };
-    auto page_of = [&](int t, bool& bad) {                 // (t never falls back by a whole load)
-      if (t - tb == 64) {
-        tb = t;
-        load_pages();
-      }
-      const int pg = __builtin_amdgcn_readlane(pages, t - tb);
-      bad = pg < 0;
-      return bad ? 0 : pg;
+    auto slot_of = [&](int t, int offset, int pg) {        // first of those rows in the pool
+      return (((int64_t)max(pg, 0) * p.G + g) << log_p) + ((t * TILE + offset) & ((1 << log_p) - 1));
     };
-    load_pages();
-    auto slot_of = [&](int t, int pg) {                    // first row of those in the pool
-      return (((int64_t)pg * p.G + g) << p.log_p) + ((t * TILE + ROWS * w) & ((1 << p.log_p) - 1));
-    };
-
-    // ---- loads of a tile: key codes (KL lanes a row) and their pairs; value codes (a lane 8 columns of ST x 4 rows) and the pairs
-    unsigned kreg[UL], kmeta;
-    const int krow = lane / KL, kpart = lane % KL;
-    const int kw = p.Rk >> 3, vw = p.Rv >> 3;
-    const unsigned klane = krow * kw + kpart * UL;
-    auto load_k = [&](int64_t slot) {
-      const unsigned* src = p.kc + slot * kw + klane;
-      if (kw == KL * UL) {
-#pragma unroll
-        for (int i = 0; i < UL; ++i) kreg[i] = src[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < UL; ++i) kreg[i] = kpart * UL + i < kw ? src[i] : 0u;
-      }
-      kmeta = (p.km + slot)[(unsigned)krow];
-    };
-    unsigned vreg[ST][4], smk, smv;
-    const int vcol = lane & (64 / S - 1), vsub = lane / (64 / S);
-    const unsigned vlane = 4 * vsub * vw + vcol, srow = lane & (ROWS - 1);
-    auto load_v = [&](int64_t slot) {
-      const unsigned* src = p.vc + slot * vw;              // (rows by their scalar address, the lane's part of it a constant)
-      if (vcol < vw) {
-#pragma unroll
-        for (int st = 0; st < ST; ++st)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) vreg[st][k] = (src + (4 * S * st + k) * vw)[vlane];
-      }
-      smk = (p.km + slot)[srow];
-      smv = (p.vm + slot)[srow];
-    };
-#pragma unroll
-    for (int st = 0; st < ST; ++st)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) vreg[st][k] = 0;
-
-    bool bad0, bad1, bad2, badv = false;                   // of tiles t, t + 1, t + 2, t - 1
-    int pg0 = page_of(t0, bad0);
-    load_k(slot_of(t0, pg0));
-    load_v(slot_of(t0, pg0));
-    int pg1 = page_of(t0 + 1, bad1), pg2 = page_of(t0 + 2, bad2);
-
-    // ---- fold the query into B: row m of an A fragment is (head m / 16 of the block's two, column (pair, cos or sin)), a lane has 8
-    // values of r
-    h16x8 F[MB][NKS];
-    float hs;                                              // (softmax lane: head lane >> 4) factor of the finished product
-    {
-      // the query is scaled to 16 .. 32 by a power of two, so that the fold's rounding to fp16 (2^-11 of each element: a score is a
-      // sum of 128 Rk independent ones) meets no subnormals; hs takes the factor back (2^10: the latents are held as (c - z) 2^-10)
-      const int e = n & 3, pair = 8 * w + 4 * ((n >> 3) & 1) + 2 * ((n >> 2) & 1) + (e >> 1);
-      const h16x8* frag = reinterpret_cast<const h16x8*>(p.bfrag) + ((int64_t)(gv * 8 + w) * MB * NKS) * 64 + lane;
-      const h16* q = p.q + (int64_t)b * p.sq_b + (int64_t)h0 * p.sq_h;
-      const int hq = min(lane >> 4, nh - 1);
-      const h16x8 q8 = *reinterpret_cast<const h16x8*>(q + hq * p.sq_h + 8 * (lane & 15));
-      h16 qa[MB], qb[MB];
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        const h16* qr = q + min(2 * mb + (n >> 4), nh - 1) * p.sq_h + pair;
-        qa[mb] = qr[0];
-        qb[mb] = qr[64];
-      }
-      float big = 0.f;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) big = fmaxf(big, fabsf((float)q8[d]));
-      big = row_max16(big);
-      int ex = 0;                                          // exponent of the largest, less 4
-      if (big > 0.f && big < INFINITY) ex = (int)(__builtin_bit_cast(unsigned, big) >> 23) - 131;
-      hs = p.scale * __builtin_bit_cast(float, (unsigned)(ex + 137) << 23);
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        const int e0 = __builtin_amdgcn_readlane(ex, 32 * mb), e1 = __builtin_amdgcn_readlane(ex, 32 * mb + 16);
-        const float f = __builtin_bit_cast(float, (unsigned)(127 - ((n >> 4) ? e1 : e0)) << 23);
-        const float q1 = (float)qa[mb] * f, q2 = (float)qb[mb] * f;
-        const float own_f = (e & 1) ? -q1 : q1;
-#pragma unroll
-        for (int kb = 0; kb < NKS; ++kb) {
-          // lanes of a (cos, sin) pair hold B[r, i] and B[r, i + 64]: each takes the other's from its neighbour
-          const u32x4 own = __builtin_bit_cast(u32x4, frag[(mb * NKS + kb) * 64]);
-          u32x4 oth;
-#pragma unroll
-          for (int d = 0; d < 4; ++d) oth[d] = __builtin_amdgcn_update_dpp(0, own[d], 0xB1, 0xf, 0xf, false);   // quad_perm [1, 0, 3, 2]
-          const h16x8 a = __builtin_bit_cast(h16x8, own), c = __builtin_bit_cast(h16x8, oth);
-#pragma unroll
-          for (int d = 0; d < 8; ++d) F[mb][kb][d] = (h16)fmaf((float)a[d], own_f, (float)c[d] * q2);
-        }
-      }
-    }
-
-    // ---- rotation state: cos / sin of this lane's 4 pairs at position (block's first) + n, and (in LDS) of a step of 32
-    float tc[4], ts[4];
-    auto turn = [&](double a, float& c, float& s) {        // v_sin / v_cos take revolutions: off by 1.2e-7 at most
-      const double rev = a * 0.15915494309189533577;
-      const float f = (float)(rev - rint(rev));
-      c = __builtin_amdgcn_cosf(f);
-      s = __builtin_amdgcn_sinf(f);
-    };
-    auto start_angles = [&](int t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const double wi = p.inv_freq[8 * w + 4 * (i >> 1) + 2 * hi + (i & 1)];
-        turn((double)((int64_t)t * TILE + n - qp) * wi, tc[i], ts[i]);
-      }
-    };
-    if (n < 4) {
-      float c, s;
-      turn(32.0 * (double)p.inv_freq[8 * w + 4 * (n >> 1) + 2 * hi + (n & 1)], c, s);
-      float* o = reinterpret_cast<float*>(smem + L::STEP) + w * 16 + hi * 8 + n;
-      o[0] = c;
-      o[4] = s;
-    }
-
     // eight codes -> fp16 (c - z) 2^-10, exactly for whole z: the bits of a code in the low bits of a half are the subnormal c 2^-24,
-    // four bits up c 2^-20; one packed multiply-add scales it and takes z off.  Order in the word pair: nibbles 0 4 | 1 5 | 2 6 | 3 7.
-    // (Subnormals straight into the matrix unit, and z taken off at the end, would be less work: but it aligns their products as if
-    // they were normal, and loses bits of the small ones: errors of 2^-19 of a sum, measured.)
+    // four bits up c 2^-20; one packed multiply-add scales it and takes z off.  (Subnormals straight into the matrix unit, and z taken
+    // off at the end, would be less work: but it aligns their products as if they were normal, and loses bits of the small ones:
+    // errors of 2^-19 of a sum, measured.)
     const h16x2 m0 = {(h16)16384.f, (h16)16384.f}, m1 = {(h16)1024.f, (h16)1024.f};
     auto scaled = [&](unsigned bits, h16x2 mul, h16x2 z) { return __builtin_elementwise_fma(__builtin_bit_cast(h16x2, bits), mul, z); };
-    auto dequant_k = [&](int buf) {
-      const h16x2 meta = __builtin_bit_cast(h16x2, kmeta);
-      const h16 mz = meta[1] * (h16)(-0.0009765625f);
-      const h16x2 z2 = {mz, mz};
-      char* dst = smem + buf * (TILE * L::XS) + (ROWS * w + krow) * L::XS + kpart * UL * 16;
-#pragma unroll
-      for (int i = 0; i < UL; ++i) {
+
+    if (w < 8) {
+      // ================================================ scores
+      const int n = lane & 31, hi = lane >> 5;
+      unsigned kreg[UL], kmeta;
+      int tb = t0, pages = load_pages(t0, KROWS * w);
+      auto load_k = [&](int t) {
+        if (t - tb == 64) {
+          tb = t;
+          pages = load_pages(t, KROWS * w);
+        }
+        const int64_t slot = slot_of(t, KROWS * w, __builtin_amdgcn_readlane(pages, t - tb));
+        int ln = lane;
+        pa_opaque(ln);
+        const int krow = ln / KL, kpart = ln % KL;         // (a lane behind the row's end takes its last words: F is zero there)
+        lane_words<UL>(kreg, p.kc + slot * kw, 4 * (unsigned)(krow * kw + min(kpart * UL, kw - UL)));
+        kmeta = lane_word(p.km + slot, 4 * (unsigned)krow);
+      };
+      auto dequant_word = [&](char* dst, int i) {          // (order in a word's 16 bytes: nibbles 0 4 | 1 5 | 2 6 | 3 7)
+        const h16 mz = __builtin_bit_cast(h16x2, kmeta)[1] * (h16)(-0.0009765625f);
+        const h16x2 z2 = {mz, mz};
         const unsigned v = kreg[i], v8 = v >> 8;
         u32x4 o;
         o[0] = __builtin_bit_cast(unsigned, scaled(v & 0x000F000Fu, m0, z2));
@@ -370,64 +297,144 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_kernel(PagedAttnPara
         o[2] = __builtin_bit_cast(unsigned, scaled(v8 & 0x000F000Fu, m0, z2));
         o[3] = __builtin_bit_cast(unsigned, scaled(v8 & 0x00F000F0u, m1, z2));
         *reinterpret_cast<u32x4*>(dst + 16 * i) = o;
-      }
-    };
-    dequant_k(t0 & 1);
-    load_k(slot_of(t0 + 1, pg1));
-    start_angles(t0);
-
-    // ---- running state of this wave's positions (softmax lane: head lane >> 4, position lane & 15)
-    float m = -INFINITY, lsum = 0.f, vn = 0.f;
-    f32x4 acc[8];                                          // [column of the lane's 8][head], times 2^-10 2^15 / vn
-#pragma unroll
-    for (int c = 0; c < 8; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    __syncthreads();
-
-    // scores of tile t, this wave's pairs; then the codes of tile t + 1 and the loads of t + 2
-    auto scores = [&](int t) {
-      const int buf = t & 1;
-      if (t != t0 && ((t - t0) & 31) == 0) start_angles(t);
-      // A unit is one 32-position block of one pair of heads: NKS dependent matrix instructions, then its dot products in the shadow
-      // of the next unit's
-      constexpr int U = NB * MB;
-      h16x8 x[NKS];
-      f32x16 y[2];
-      float part[2][NH];
-      const char* const xt = smem + buf * (TILE * L::XS) + n * L::XS + hi * 16;
-      auto load_x = [&](int nb) {
-#pragma unroll
-        for (int kb = 0; kb < NKS; ++kb) x[kb] = *reinterpret_cast<const h16x8*>(xt + 32 * nb * L::XS + kb * 32);
       };
-      auto product = [&](int u) {
-        f32x16 v = {};
-#pragma unroll
-        for (int kb = 0; kb < NKS; ++kb) v = __builtin_amdgcn_mfma_f32_32x32x16_f16(F[u % MB][kb], x[kb], v, 0, 0, 0);
-        y[u & 1] = v;
-        if (u % MB == MB - 1 && u / MB + 1 < NB) load_x(u / MB + 1);
+      auto dequant_dst = [&](int buf, int ln) {
+        return smem + buf * (TILE * L::XS) + (KROWS * w + ln / KL) * L::XS + ln % KL * UL * 16;
       };
-      load_x(0);
-      product(0);
+      load_k(t0);
+
+      // ---- fold the query into B: row m of an A fragment is (head m / 16 of the block's two, column (pair, cos or sin)), a lane has 8
+      // values of r.  The query is scaled to 16 .. 32 by a power of two, so that the fold's rounding to fp16 (2^-11 of each element: a
+      // score is a sum of 128 Rk independent ones) meets no subnormals; the value waves take the factor back.
+      h16x8 F[MB][NKS];
+      {
+        const int e = n & 3, pair = 8 * w + 4 * ((n >> 3) & 1) + 2 * ((n >> 2) & 1) + (e >> 1);
+        const h16x8* frag = reinterpret_cast<const h16x8*>(p.bfrag) + ((int64_t)(gv * 8 + w) * MB * NKS) * 64 + lane;
+        const h16* q = p.q + (int64_t)b * p.sq_b + (int64_t)h0 * p.sq_h;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int nb = u / MB, mb = u % MB;
-        if (u + 1 < U) product(u + 1);
+        for (int mb = 0; mb < MB; ++mb)                    // (all requests first; the fold is in place)
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
-          float s0 = 0.f, s1 = 0.f;
+          for (int kb = 0; kb < NKS; ++kb) F[mb][kb] = frag[(mb * NKS + kb) * 64];
+        h16 qa[MB], qb[MB];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s0 = fmaf(y[u & 1][8 * d + 2 * i], tc[i], s0);
-            s1 = fmaf(y[u & 1][8 * d + 2 * i + 1], ts[i], s1);
-          }
-          part[nb & 1][2 * mb + d] = s0 + s1;
+        for (int mb = 0; mb < MB; ++mb) {
+          const h16* qr = q + min(2 * mb + (n >> 4), nh - 1) * p.sq_h + pair;
+          qa[mb] = qr[0];
+          qb[mb] = qr[64];
         }
-        if (mb == MB - 1) {
-          const f32x4 rc = step[0], rs = step[1];
+        const int ex = pa_query_exponent(q, p.sq_h, nh, lane);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float c = tc[i];
-            tc[i] = c * rc[i] - ts[i] * rs[i];
-            ts[i] = c * rs[i] + ts[i] * rc[i];
+        for (int mb = 0; mb < MB; ++mb) {
+          const int e0 = __builtin_amdgcn_readlane(ex, 32 * mb), e1 = __builtin_amdgcn_readlane(ex, 32 * mb + 16);
+          const float f = __builtin_bit_cast(float, (unsigned)(127 - ((n >> 4) ? e1 : e0)) << 23);
+          const float q1 = (float)qa[mb] * f, q2 = (float)qb[mb] * f;
+          const float own_f = (e & 1) ? -q1 : q1;
+#pragma unroll
+          for (int kb = 0; kb < NKS; ++kb) {
+            // lanes of a (cos, sin) pair hold B[r, i] and B[r, i + 64]: each takes the other's from its neighbour
+            const u32x4 own = __builtin_bit_cast(u32x4, F[mb][kb]);
+            u32x4 oth;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) oth[d] = __builtin_amdgcn_update_dpp(0, own[d], 0xB1, 0xf, 0xf, false);   // quad_perm [1, 0, 3, 2]
+            const h16x8 x = __builtin_bit_cast(h16x8, own), c = __builtin_bit_cast(h16x8, oth);
+#pragma unroll
+            for (int d = 0; d < 8; ++d) F[mb][kb][d] = (h16)fmaf((float)x[d], own_f, (float)c[d] * q2);
+            pa_opaque(F[mb][kb]);                          // (done here: not, at the cost of twice the registers, at its use)
+          }
+        }
+      }
+
+      // ---- rotation state: cos / sin of this lane's 4 pairs at position (block's first) + n, and (in LDS) of a step of 32
+      float tc[4], ts[4];
+      auto turn = [&](double a, float& c, float& s) {      // v_sin / v_cos take revolutions: off by 1.2e-7 at most
+        const double rev = a * 0.15915494309189533577;
+        const float f = (float)(rev - rint(rev));
+        c = __builtin_amdgcn_cosf(f);
+        s = __builtin_amdgcn_sinf(f);
+      };
+      auto start_angles = [&](int t) {
+        int ln = lane;
+        pa_opaque(ln);
+        const int at_n = (ln & 31) - qp;
+        const unsigned pair0 = 4 * (8 * w + 2 * (ln >> 5));
+        const double l = (double)(t * TILE + at_n);        // (below 2^30 + 2^30 in size)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const double wi = __builtin_bit_cast(float, lane_word(reinterpret_cast<const unsigned*>(p.inv_freq), pair0 + 16 * (i >> 1) + 4 * (i & 1)));
+          turn(l * wi, tc[i], ts[i]);
+        }
+      };
+      if (n < 4) {
+        float c, s;
+        turn(32.0 * (double)p.inv_freq[8 * w + 4 * (n >> 1) + 2 * hi + (n & 1)], c, s);
+        float* o = reinterpret_cast<float*>(smem + L::STEP) + w * 16 + hi * 8 + n;
+        o[0] = c;
+        o[4] = s;
+      }
+#pragma unroll
+      for (int i = 0; i < UL; ++i) dequant_word(dequant_dst(t0 & 1, lane), i);
+      load_k(t0 + 1);
+      start_angles(t0);
+      __syncthreads();
+
+      int exact = 32;                                      // tiles until the angles are computed anew
+#pragma clang loop unroll(disable)
+      for (int t = t0; t < t1; ++t) {
+        const int buf = t & 1;
+        if (--exact < 0) {
+          start_angles(t);
+          exact = 31;
+        }
+        // The tile's blocks one after the other: NKS steps, each the matrix instructions of one 16-column piece of x (read from LDS two
+        // steps ahead) with some of the wave's other work in their shadow -- the next tile's codes, the rotation, the finished
+        // partial scores -- then the block's dot products (the other score wave of the SIMD has the matrix pipe meanwhile).  The
+        // barriers keep this order: left to itself hipcc reads far ahead and spills.
+        // (What a lane's number gives -- addresses -- is made anew in every tile: kept, it would cost registers that F and y need.)
+        int ln = lane;
+        pa_opaque(ln);
+        const char* const xt = smem + buf * (TILE * L::XS) + (ln & 31) * L::XS + (ln >> 5) * 16;
+        char* const kdst = dequant_dst(buf ^ 1, ln);
+        float* const rdst = red + ((buf * 8 + w) * NH) * TILE + ln;
+        const f32x4* const step = reinterpret_cast<const f32x4*>(smem + L::STEP) + w * 4 + (ln >> 5) * 2;
+        constexpr int XD = 3;
+        h16x8 x[XD];
+        auto read_x = [&](int i) { x[i % XD] = *reinterpret_cast<const h16x8*>(xt + 32 * (i / NKS) * L::XS + (i % NKS) * 32); };
+        float part[2][NH];
+        read_x(0);
+        read_x(1);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          f32x16 y[MB];
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) y[mb] = f32x16{};
+#pragma unroll
+          for (int kb = 0; kb < NKS; ++kb) {
+            const int i = nb * NKS + kb;
+            if (i + 2 < NB * NKS) read_x(i + 2);
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) y[mb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(F[mb][kb], x[i % XD], y[mb], 0, 0, 0);
+            if (nb == 0 && kb < UL) dequant_word(kdst, kb);
+            if (nb == (UL == NKS ? 1 : 0) && kb == (UL == NKS ? 0 : UL)) load_k(t + 2);   // (behind the range: page 0, not used)
+            if (nb > 0 && kb == 0) {
+              const f32x4 rc = step[0], rs = step[1];
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                const float c = tc[d];
+                tc[d] = c * rc[d] - ts[d] * rs[d];
+                ts[d] = c * rs[d] + ts[d] * rc[d];
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int j = 0; j < NH; ++j) {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              s0 = fmaf(y[j / 2][8 * (j & 1) + 2 * d], tc[d], s0);
+              s1 = fmaf(y[j / 2][8 * (j & 1) + 2 * d + 1], ts[d], s1);
+            }
+            part[nb & 1][j] = s0 + s1;
           }
           if (nb & 1) {
 #pragma unroll
@@ -435,153 +442,221 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_kernel(PagedAttnPara
               const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, part[0][j]),
                                                                __builtin_bit_cast(unsigned, part[1][j]), false, false);
               const unsigned lo = sw[0], up = sw[1];       // (plain values first: a bit cast of a vector's element takes element 0)
-              red[((buf * 8 + w) * 4 + j) * TILE + 32 * (nb - 1) + lane] = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, up);
+              rdst[j * TILE + 32 * (nb - 1)] = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, up);
             }
           }
         }
-        if (u + 1 < U) {
+        {                                                  // on to the next tile's first block
+          const f32x4 rc = step[0], rs = step[1];
 #pragma unroll
-          for (int kb = 0; kb < NKS; ++kb) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                 // one matrix instruction,
-            __builtin_amdgcn_sched_group_barrier(0x002, (32 + NKS - 1) / NKS, 0);   // its share of the vector instructions
+          for (int d = 0; d < 4; ++d) {
+            const float c = tc[d];
+            tc[d] = c * rc[d] - ts[d] * rs[d];
+            ts[d] = c * rs[d] + ts[d] * rc[d];
           }
         }
+        __syncthreads();
       }
-      if (t + 1 < t1) dequant_k(buf ^ 1);
-      if (t + 2 < t1) load_k(slot_of(t + 2, pg2));
-    };
-
-    // softmax and values of tile t (its scores are complete), this wave's positions; then the loads of tile t + 1
-    auto values = [&](int t) {
-      const int buf = t & 1;
-      const int head = lane >> 4, pos = lane & 15;
-      const int hsafe = NH == 4 ? head : head & (NH - 1), psafe = pos & (ROWS - 1);
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) s += red[((buf * 8 + k) * 4 + hsafe) * TILE + ROWS * w + psafe];
-      const h16x2 mk = __builtin_bit_cast(h16x2, smk), mv = __builtin_bit_cast(h16x2, smv);
-      const bool valid = pos < ROWS && t * TILE + ROWS * w + pos < rows && head < NH;
-      s *= (float)mk[0] * hs;
-      if (badv) s = NAN;
-      if (!valid) s = -INFINITY;
-      const float mn = fmaxf(m, row_max16(s));
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      const float alpha = __builtin_amdgcn_exp2f(m - ref);
-      const float pr = __builtin_amdgcn_exp2f(s - ref);
-      // Weights: probability times the row's value scale, over the largest scale so far (its power of two) and times 2^15, in fp16:
-      // 2^-11 of each weight down to 2^-29 of the largest.
-      const float sv = valid ? (float)mv[0] : 0.f;
-      const float top = row_max16(fabsf(sv));
-      const float vp = fmaxf(vn, __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, top) + 0x7fffffu) & 0x7f800000u));
-      const float rv = vp > 0.f ? 32768.f * __builtin_amdgcn_rcpf(vp) : 0.f;      // (of a power of two: exact)
-      const h16 wt = (h16)(pr * (sv * rv));
-      const float shrink = alpha * vn * rv * (1.f / 32768.f);
-      const bool moved = mn != m || vp != vn;
-      lsum = lsum * alpha + pr;
-      m = mn;
-      vn = vp;
-      wgt[lane] = wt;
-      if (lane < 16) wgt[64 + lane] = valid ? mv[1] * (h16)(-0.0009765625f) : (h16)0.f;
-      if (__ballot(moved)) {
-#pragma unroll
-        for (int j = 0; j < NH; ++j) {
-          const float a = lane_value(shrink, 16 * j);
-#pragma unroll
-          for (int c = 0; c < 8; ++c) acc[c][j] *= a;
+      __syncthreads();                                     // (the values of the last tile)
+      __syncthreads();                                     // (the statistics)
+      __syncthreads();                                     // (the slabs)
+    } else {
+      // ================================================ softmax and values: positions 32 v .. 32 v + 31 of a tile
+      const int v = w - 8;
+      h16* const wgt = reinterpret_cast<h16*>(smem + L::WGT) + v * 160;
+      // A lane is (head lane >> 4, positions lane & 15 and 16 more) in the softmax, and (rows 8 (lane >> 4) .., words (lane & 15) + 16 cc) in
+      // the values; all of it is made anew in every tile, as in the scores.
+      unsigned vreg[NC][8], smk[2], smv[2];
+      int tb = t0, pages0 = load_pages(t0, 32 * v), pages1 = load_pages(t0, 32 * v + 16);
+      bool bad0, bad1;                                     // of the tile that is loaded
+      const unsigned* vsrc;                                // its values, this lane's first word
+      auto next_tile = [&](int t) {                        // (behind the range: page 0 again, whose rows are masked)
+        if (t - tb == 64) {
+          tb = t;
+          pages0 = load_pages(t, 32 * v);
+          pages1 = load_pages(t, 32 * v + 16);
         }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int st = 0; st < ST; ++st) {
-        const h16x4 a = *reinterpret_cast<const h16x4*>(wgt + (lane & 3) * 16 + 4 * (st * S + vsub));
-        const h16x4 z4 = *reinterpret_cast<const h16x4*>(wgt + 64 + 4 * (st * S + vsub));
-        const h16x2 z01 = {z4[0], z4[1]}, z23 = {z4[2], z4[3]};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const unsigned sel = half ? 0x07060302u : 0x05040100u;
-          const unsigned p01 = __builtin_amdgcn_perm(vreg[st][1], vreg[st][0], sel);
-          const unsigned p23 = __builtin_amdgcn_perm(vreg[st][3], vreg[st][2], sel);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const unsigned mask = c & 1 ? 0x00F000F0u : 0x000F000Fu;
-            const h16x2 v01 = scaled((c & 2 ? p01 >> 8 : p01) & mask, c & 1 ? m1 : m0, z01);
-            const h16x2 v23 = scaled((c & 2 ? p23 >> 8 : p23) & mask, c & 1 ? m1 : m0, z23);
-            const h16x4 v = {v01[0], v01[1], v23[0], v23[1]};
-            acc[4 * half + c] = __builtin_amdgcn_mfma_f32_4x4x4f16(a, v, acc[4 * half + c], 0, 0, 0);
-          }
+        const int pg0 = __builtin_amdgcn_readlane(pages0, t - tb), pg1 = __builtin_amdgcn_readlane(pages1, t - tb);
+        bad0 = pg0 < 0;
+        bad1 = pg1 < 0;
+        const int64_t slot0 = slot_of(t, 32 * v, pg0), slot1 = slot_of(t, 32 * v + 16, pg1);
+        int ln = lane;
+        pa_opaque(ln);
+        vsrc = p.vc + ((ln & 32 ? slot1 : slot0) + (ln & 16) / 2) * vw + (ln & 15);
+        const unsigned pos4 = 4 * (ln & 15);
+        smk[0] = lane_word(p.km + slot0, pos4);
+        smk[1] = lane_word(p.km + slot1, pos4);
+        smv[0] = lane_word(p.vm + slot0, pos4);
+        smv[1] = lane_word(p.vm + slot1, pos4);
+      };
+      auto load_v = [&](int cc) {                          // (a column behind the row's end is read in front of it: never used)
+        const unsigned* src = vsrc + 16 * cc;
+        if (cc == NC - 1) {
+          int vcol = lane & 15;
+          pa_opaque(vcol);
+          if (16 * cc + vcol >= vw) src = vsrc - vcol;
         }
-      }
-      if (t + 1 < t1) load_v(slot_of(t + 1, pg0));
-    };
-
-    for (int t = t0; t <= t1; ++t) {                       // (the last turn: only the values of the last tile)
-      if (w >= 4 && t > t0) values(t - 1);
-      if (t < t1) scores(t);
-      if (w < 4 && t > t0) values(t - 1);
-      badv = bad0;
-      pg0 = pg1;
-      bad0 = bad1;
-      pg1 = pg2;
-      bad1 = bad2;
-      pg2 = page_of(t + 3, bad2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          vreg[cc][i] = *src;
+          src += vw;
+          asm volatile("" : "+v"(src));
+        }
+      };
+      next_tile(t0);
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) load_v(cc);
+      // factor of a finished product of head lane >> 4 (2^10: the latents are held as (c - z) 2^-10)
+      const int ex = pa_query_exponent(p.q + (int64_t)b * p.sq_b + (int64_t)h0 * p.sq_h, p.sq_h, nh, lane);
+      const float hs = p.scale * __builtin_bit_cast(float, (unsigned)(ex + 137) << 23);
+      float m = -INFINITY, lsum = 0.f;
+      f32x4 acc[NC][8];                                    // [chunk][column of the lane's 8][head], times 2^-10 2^8; the same in all four vq
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[cc][c] = f32x4{0.f, 0.f, 0.f, 0.f};
       __syncthreads();
-    }
+      __syncthreads();                                     // (the scores of the first tile)
 
-    // ---- join the eight waves: slabs of every (wave, subset) through LDS, summed in a fixed order
-    float* const slab = reinterpret_cast<float*>(smem);
-    float* const stat = reinterpret_cast<float*>(smem + L::STAT);
-    lsum = row_sum16(lsum);
-    if ((lane & 15) == 0) {
-      float* o = stat + (w * 4 + (lane >> 4)) * 4;
-      o[0] = m;
-      o[1] = vn;
-      o[2] = lsum;
-    }
-    __syncthreads();
-    // lane (wave k, head j) of every wave: the maximum of the eight, each wave's factor, the sum of the eight
-    {
-      const int k = (lane >> 2) & 7, j = lane & 3;
-      const float* o = stat + (k * 4 + j) * 4;
+      for (int t = t0; t < t1; ++t) {
+        int ln = lane;
+        pa_opaque(ln);
+        const int head = ln >> 4, pos = ln & 15;
+        const float* const rt = red + ((t & 1) * 8 * NH + (NH == 4 ? head : head & (NH - 1))) * TILE + 32 * v + pos;
+        float part[2][8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) part[h][k] = rt[k * NH * TILE + 16 * h];
+        float sc[2], sw[2], sv[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float s = ((part[h][0] + part[h][1]) + (part[h][2] + part[h][3])) + ((part[h][4] + part[h][5]) + (part[h][6] + part[h][7]));
+          const h16x2 mk = __builtin_bit_cast(h16x2, smk[h]), mv = __builtin_bit_cast(h16x2, smv[h]);
+          const bool valid = t * TILE + 32 * v + 16 * h + pos < rows && head < NH;
+          s *= (float)mk[0] * hs;
+          if (h ? bad1 : bad0) s = NAN;
+          // The value's scale goes into the weight, and the maximum is that of s + log2 |scale|.  The weights' reference m follows it
+          // only when it has grown by more than 2^7: weights then lie in 0 .. 2^15 and are held in fp16 to 2^-11 of themselves down
+          // to 2^-22 of the largest, whatever the scales are, and the accumulators are hardly ever rescaled.  (The probabilities'
+          // own sum is kept in 32 bits against the same reference, within 2^40 of 1: scales below 2^-30, that is 0, count as 2^-30.)
+          sv[h] = valid ? (float)mv[0] : 0.f;
+          const float sa = fabsf(sv[h]) < 0x1p-30f ? 0x1p-30f : fabsf(sv[h]);
+          sc[h] = valid ? s : -INFINITY;
+          sw[h] = sc[h] + __builtin_amdgcn_logf(sa);
+          if (ln < 16) wgt[128 + 16 * h + ln] = valid ? mv[1] * (h16)(-0.0009765625f) : (h16)0.f;
+        }
+        const float top = row_max16(fmaxf(sw[0], sw[1]));
+        if (__ballot(top > m + 7.f)) {                     // (m is -inf at first: the first finite maximum is taken)
+          const float mn = top > m + 7.f ? top : m;
+          const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+          lsum *= alpha;
+          m = mn;
+#pragma unroll
+          for (int j = 0; j < NH; ++j) {
+            const float a = lane_value(alpha, 16 * j);
+#pragma unroll
+            for (int cc = 0; cc < NC; ++cc)
+#pragma unroll
+              for (int c = 0; c < 8; ++c) acc[cc][c][j] *= a;
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float we = __builtin_amdgcn_exp2f(sw[h] - (ref - 8.f));
+          wgt[head * 32 + 16 * h + pos] = (h16)(sv[h] == 0.f ? 0.f : __builtin_copysignf(we, sv[h]));
+          lsum += __builtin_amdgcn_exp2f(sc[h] - ref);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const h16x8 a = *reinterpret_cast<const h16x8*>(wgt + (ln & 3) * 32 + 8 * head);
+        const u32x4 z4 = *reinterpret_cast<const u32x4*>(wgt + 128 + 8 * head);
+        next_tile(t + 1);                                  // (its values are requested chunk by chunk, as the registers come free)
+#pragma unroll
+        for (int cc = 0; cc < NC; ++cc) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const unsigned sel = half ? 0x07060302u : 0x05040100u;
+            unsigned w0[4], w8[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              w0[i] = __builtin_amdgcn_perm(vreg[cc][2 * i + 1], vreg[cc][2 * i], sel);
+              w8[i] = w0[i] >> 8;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              u32x4 x;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                x[i] = __builtin_bit_cast(unsigned, scaled((c & 2 ? w8[i] : w0[i]) & (c & 1 ? 0x00F000F0u : 0x000F000Fu),
+                                                           c & 1 ? m1 : m0, __builtin_bit_cast(h16x2, (unsigned)z4[i])));
+              acc[cc][4 * half + c] =
+                  __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(h16x8, x), acc[cc][4 * half + c], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          load_v(cc);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+      }
+
+      // ---- join the four waves: the slabs of each through LDS, summed in a fixed order
+      lsum = row_sum16(lsum);
+      int le = lane;
+      pa_opaque(le);
+      const int ecol = le & 15, eq = le >> 4;
+      if (ecol == 0) {
+        float* o = stat + (v * 4 + eq) * 2;
+        o[0] = m;
+        o[1] = lsum;
+      }
+      __syncthreads();
+      // lane (wave k, head j): the maximum of the four, each wave's factor, the sum of the four
+      const int k = (le >> 2) & 3, j = le & 3;
+      const float* o = stat + (k * 4 + j) * 2;
       const float mk = o[0];
       float top = mk;
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+      for (int x = 4; x < 16; x <<= 1) top = fmaxf(top, pa_other(top, le ^ x));
       const float a = __builtin_amdgcn_exp2f(mk - (top == -INFINITY ? 0.f : top));
-      float sum = a * o[2];
+      float sum = a * o[1];
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor(sum, x, 64);
-      const float mine = a * o[1] * (1.f / 32.f);
-      if (w == 0 && lane < 4) {
-        stat[128 + j] = sum;
-        stat[132 + j] = top;
+      for (int x = 4; x < 16; x <<= 1) sum += pa_other(sum, le ^ x);
+      const float mine = a * 4.f;                          // (2^10 2^-8)
+      if (v == 0 && le < 4) {
+        stat[32 + j] = sum;
+        stat[36 + j] = top;
       }
 #pragma unroll
-      for (int jj = 0; jj < NH; ++jj) {
-        const float f = lane_value(mine, 4 * w + jj);
-        if (vcol < vw) {
-          float* d = slab + (w * S + vsub) * (PA_SLAB / S) + jj * (512 / S) + 8 * vcol;
-          *reinterpret_cast<f32x4*>(d) = f32x4{acc[0][jj] * f, acc[1][jj] * f, acc[2][jj] * f, acc[3][jj] * f};
-          *reinterpret_cast<f32x4*>(d + 4) = f32x4{acc[4][jj] * f, acc[5][jj] * f, acc[6][jj] * f, acc[7][jj] * f};
-        }
+      for (int jj = 0; jj < NH; ++jj) {                    // lanes vq = jj write head jj
+        const float f = lane_value(mine, 4 * v + jj);
+#pragma unroll
+        for (int cc = 0; cc < NC; ++cc)
+          if (eq == jj && 16 * cc + ecol < vw) {
+            float* d = slab + (v * 4 + jj) * 512 + 8 * (16 * cc + ecol);
+            *reinterpret_cast<f32x4*>(d) = f32x4{acc[cc][0][jj] * f, acc[cc][1][jj] * f, acc[cc][2][jj] * f, acc[cc][3][jj] * f};
+            *reinterpret_cast<f32x4*>(d + 4) = f32x4{acc[cc][4][jj] * f, acc[cc][5][jj] * f, acc[cc][6][jj] * f, acc[cc][7][jj] * f};
+          }
       }
+      __syncthreads();
     }
-    __syncthreads();
     const bool whole = t0 == 0 && t1 == nt;                // this workgroup has all of the sequence: the result itself
     const bool poison = pa_bad_len(p, b);
     const int64_t slot = (int64_t)blockIdx.x + b * GV + gv;      // (grows from piece to piece: a slot of its own for each)
     for (int i = tid; i < nh * p.Rv; i += PA_THREADS) {
       const int j = i / p.Rv, c = i - j * p.Rv;
-      const float* o = slab + j * (512 / S) + c;
+      const float* o = slab + j * 512 + c;
       float v = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8 * S; ++k) v += o[k * (PA_SLAB / S)];
-      if (whole) p.ctx[((int64_t)b * p.H + h0 + j) * p.Rv + c] = (h16)(poison ? NAN : v / stat[128 + j]);
+      for (int k = 0; k < 4; ++k) v += o[k * 2048];
+      if (whole) p.ctx[((int64_t)b * p.H + h0 + j) * p.Rv + c] = (h16)(poison ? NAN : v / stat[32 + j]);
       else p.part[(int64_t)p.slots * 8 + (slot * 4 + j) * p.Rv + c] = v;
     }
     if (!whole && tid < nh) {
-      p.part[(slot * 4 + tid) * 2] = stat[132 + tid];
-      p.part[(slot * 4 + tid) * 2 + 1] = stat[128 + tid];
+      p.part[(slot * 4 + tid) * 2] = stat[36 + tid];
+      p.part[(slot * 4 + tid) * 2 + 1] = stat[32 + tid];
     }
     if (p.direct || at >= end) break;
     if (gv == GV - 1) {
@@ -598,31 +673,34 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_kernel(PagedAttnPara
   }
 }
 
-template <int NKS, int S, int NH>
+template <int NKS, int NC, int NH>
 int pa_launch1(const PagedAttnParams& p, int wgs, hipStream_t stream) {
-  auto kern = paged_attn_kernel<NKS, S, NH>;
-  const int rc = palu_func_max_lds(reinterpret_cast<const void*>(kern), PaLds<NKS>::BYTES);
+  auto kern = paged_attn_kernel<NKS, NC, NH>;
+  constexpr int lds = PaLds<NKS, NH>::BYTES;
+  const int rc = palu_func_max_lds(reinterpret_cast<const void*>(kern), lds);
   if (rc != PALU_OK) return rc;
-  hipLaunchKernelGGL(kern, dim3(wgs), dim3(PA_THREADS), PaLds<NKS>::BYTES, stream, p);
+  hipLaunchKernelGGL(kern, dim3(wgs), dim3(PA_THREADS), lds, stream, p);
   PALU_LAUNCH_CHECK();
   return PALU_OK;
 }
-template <int NKS, int S>
+template <int NKS, int NC>
 int pa_launch2(const PagedAttnParams& p, int heads, int wgs, hipStream_t stream) {
   if constexpr (NKS <= 8)
-    if (heads == 4) return pa_launch1<NKS, S, 4>(p, wgs, stream);
-  return pa_launch1<NKS, S, 2>(p, wgs, stream);
+    if (heads == 4) return pa_launch1<NKS, NC, 4>(p, wgs, stream);
+  return pa_launch1<NKS, NC, 2>(p, wgs, stream);
 }
 template <int NKS>
-int pa_launch3(const PagedAttnParams& p, int subsets, int heads, int wgs, hipStream_t stream) {
-  if (subsets == 1) return pa_launch2<NKS, 1>(p, heads, wgs, stream);
-  if constexpr (PaLds<NKS>::TILE == 128)                   // (8 positions a wave: two rows of 4 side by side at most)
-    if (subsets == 4) return pa_launch2<NKS, 4>(p, heads, wgs, stream);
-  return pa_launch2<NKS, 2>(p, heads, wgs, stream);
+int pa_launch3(const PagedAttnParams& p, int chunks, int heads, int wgs, hipStream_t stream) {
+  switch (chunks) {
+    case 1: return pa_launch2<NKS, 1>(p, heads, wgs, stream);
+    case 2: return pa_launch2<NKS, 2>(p, heads, wgs, stream);
+    case 3: return pa_launch2<NKS, 3>(p, heads, wgs, stream);
+    default: return pa_launch2<NKS, 4>(p, heads, wgs, stream);
+  }
 }
 template <int A, int B>
-int pa_launch(const PagedAttnParams& p, int nks, int subsets, int heads, int wgs, hipStream_t stream) {
-  return nks == A ? pa_launch3<A>(p, subsets, heads, wgs, stream) : pa_launch3<B>(p, subsets, heads, wgs, stream);
+int pa_launch(const PagedAttnParams& p, int nks, int chunks, int heads, int wgs, hipStream_t stream) {
+  return nks == A ? pa_launch3<A>(p, chunks, heads, wgs, stream) : pa_launch3<B>(p, chunks, heads, wgs, stream);
 }
 
 }  // namespace

@@ -2,6 +2,6 @@
 // instances compile side by side.
 #include "paged_attn_kernel.h"
 
-int palu_paged_attn_launch_mid(const void* params, int nks, int subsets, int heads, int wgs, hipStream_t stream) {
-  return pa_launch<6, 8>(*reinterpret_cast<const PagedAttnParams*>(params), nks, subsets, heads, wgs, stream);
+int palu_paged_attn_launch_mid(const void* params, int nks, int chunks, int heads, int wgs, hipStream_t stream) {
+  return pa_launch<6, 8>(*reinterpret_cast<const PagedAttnParams*>(params), nks, chunks, heads, wgs, stream);
 }
