@@ -17,68 +17,99 @@ struct AppendTensor {
   int R, lanes;                           // lanes of a row: a power of two >= R / 8, at most 64
 };
 
-// One row per `lanes` lanes, eight values a lane: one 16-byte load, the row's minimum and maximum over its lanes, eight codes, one
-// word stored.  The arithmetic is quantize_tensor's with the reference's defaults (palu/model/modules/quant.py:29-39), bit for bit
-// what palu_quantize_pack writes; two steps are shorter here and give the same bits:
+static __device__ __forceinline__ h16x2 pair_max(h16x2 a, h16x2 b) { return __builtin_elementwise_max(a, b); }
+
+// (maximum, -minimum) of a row over its lanes
+static __device__ __forceinline__ h16x2 row_extremes(h16x2 v, int lanes) {
+#define STEP(CTRL) v = pair_max(v, __builtin_bit_cast(h16x2, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false)))
+  if (lanes > 1) STEP(0xB1);               // quad_perm [1, 0, 3, 2]
+  if (lanes > 2) STEP(0x4E);               // quad_perm [2, 3, 0, 1]
+  if (lanes > 4) STEP(0x141);              // row_half_mirror: the other four of eight
+  if (lanes > 8) STEP(0x140);              // row_mirror: the other eight of sixteen
+#undef STEP
+  if (lanes > 16) v = pair_max(v, __builtin_bit_cast(h16x2, __shfl_xor(__builtin_bit_cast(int, v), 16, 64)));
+  if (lanes > 32) v = pair_max(v, __builtin_bit_cast(h16x2, __shfl_xor(__builtin_bit_cast(int, v), 32, 64)));
+  return v;
+}
+
+// One row per `lanes` lanes, eight values a lane (v; a lane behind the row's end has none), eight codes a lane.  The arithmetic is
+// quantize_tensor's with the reference's defaults (palu/model/modules/quant.py:29-39), bit for bit what palu_quantize_pack writes.
+// Three steps are shorter here and give the same bits:
 //   w / scale   = q0 + (w - q0 scale) rcp(scale), q0 = w rcp(scale): within 2^-24 of the quotient, which two 11-bit numbers cannot
 //                 bring closer than that to a rounding border of fp16 without lying on it, and there the correction is exact;
-//   the fp16 rounding of (code + zero) moves only sums beyond 2048, and those are clamped to the ends of 0 .. 15 either way.
-static __device__ __forceinline__ void append_row(const AppendTensor& t, int64_t token, int g, int64_t slot, int sub) {
-  const bool on = 8 * sub < t.R;
-  h16x8 v = {};
-  if (on) v = *reinterpret_cast<const h16x8*>(t.x + token * t.sx_t + g * t.sx_g + 8 * sub);
-  float mx = -INFINITY, mn = INFINITY;
+//   the maxima are taken of the fp16 values, and the steps behind the quotient, each of which rounds to fp16, in fp16.
+static __device__ __forceinline__ unsigned quantise8(h16x8 v, bool on, int lanes, h16x2& meta) {
+  h16x2 e = {(h16)-INFINITY, (h16)-INFINITY};
   if (on) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      mx = fmaxf(mx, (float)v[e]);
-      mn = fminf(mn, (float)v[e]);
-    }
+    const h16x2 p[4] = {{v[0], v[1]}, {v[2], v[3]}, {v[4], v[5]}, {v[6], v[7]}};
+    const h16x2 hi = pair_max(pair_max(p[0], p[1]), pair_max(p[2], p[3]));
+    const h16x2 lo = pair_max(pair_max(-p[0], -p[1]), pair_max(-p[2], -p[3]));
+    e = pair_max(h16x2{hi[0], lo[0]}, h16x2{hi[1], lo[1]});
   }
-  for (int o = t.lanes >> 1; o > 0; o >>= 1) {
-    mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    mn = fminf(mn, __shfl_xor(mn, o, 64));
-  }
+  e = row_extremes(e, lanes);
+  const float mx = (float)e[0], mn = -(float)e[1];
   const float range = fmaxf(r16(mx - mn), (float)(h16)1e-5f);
   const float scale = r16(range / 15.0f);
   const float zero = fminf(fmaxf(rintf(r16(-mn / scale)), 0.f), 15.0f);
   const float rs = __builtin_amdgcn_rcpf(scale);
+  const h16 z = (h16)zero;
   unsigned bits = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float w = (float)v[e];
-    const float q0 = w * rs;
-    const float q1 = fmaf(fmaf(-q0, scale, w), rs, q0);
-    const float c = fminf(fmaxf(rintf(r16(q1)) + zero, 0.f), 15.0f);
-    bits |= (unsigned)c << (4 * e);
+  for (int i = 0; i < 4; ++i) {
+    h16x2 c;
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const float w = (float)v[2 * i + d];
+      const float q0 = w * rs;
+      c[d] = __builtin_elementwise_rint((h16)fmaf(fmaf(-q0, scale, w), rs, q0));
+    }
+    c = __builtin_elementwise_min(__builtin_elementwise_max(c + h16x2{z, z}, h16x2{(h16)0.f, (h16)0.f}), h16x2{(h16)15.f, (h16)15.f});
+    const unsigned u = __builtin_bit_cast(unsigned, c + h16x2{(h16)1024.f, (h16)1024.f}) & 0x000F000Fu;   // 1024 + c: c in the low bits
+    bits |= ((u | u >> 12) & 0xFFu) << (8 * i);
   }
-  if (on) t.codes[slot * (t.R >> 3) + sub] = bits;
-  if (sub == 0) {
-    const h16x2 m = {(h16)scale, (h16)zero};
-    t.meta[slot] = __builtin_bit_cast(unsigned, m);
-  }
+  meta = h16x2{(h16)scale, z};
+  return bits;
 }
 
-// rows [0, T G) are the key rows, [T G, 2 T G) the value rows; a wave takes 64 / lanes rows of one of the two
+// Token rows of one group (blockIdx.y) and one of the two tensors (blockIdx.z): 64 / lanes of them a wave and turn, IT turns, whose rows
+// and places are all requested before the first is worked on.
+template <int IT>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendTensor a, AppendTensor b, const int* __restrict__ table,
                                                            int64_t st_b, int B, int max_pages, const int* __restrict__ seq,
-                                                           const int* __restrict__ pos, int64_t rows, int64_t waves_a, int G,
-                                                           int log_p, int n_pages) {
-  const int lane = threadIdx.x & 63;
-  int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const bool second = wave >= waves_a;
-  if (second) wave -= waves_a;
-  const AppendTensor& t = second ? b : a;
-  const int sub = lane & (t.lanes - 1);
-  const int64_t row = wave * (64 / t.lanes) + lane / t.lanes;
-  if (row >= rows) return;
-  const int64_t token = row / G;
-  const int g = (int)(row - token * G);
-  const int s = seq[token], p = pos[token];
-  if (s < 0 || s >= B || p < 0 || (p >> log_p) >= max_pages) return;         // a padding row, or one the table has no place for
-  const int page = table[s * st_b + (p >> log_p)];
-  if (page < 0 || page >= n_pages) return;
-  append_row(t, token, g, (((int64_t)page * G + g) << log_p) + (p & ((1 << log_p) - 1)), sub);
+                                                           const int* __restrict__ pos, int T, int G, int log_p, int n_pages) {
+  const AppendTensor& t = blockIdx.z ? b : a;
+  const int lane = threadIdx.x & 63, g = blockIdx.y;
+  const int sub = lane & (t.lanes - 1), rows = 64 / t.lanes;
+  const int64_t first = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * (IT * rows) + lane / t.lanes;
+  const bool on = 8 * sub < t.R;
+  h16x8 v[IT];
+  int s[IT], p[IT], page[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int64_t token = first + i * rows;
+    v[i] = h16x8{};
+    s[i] = p[i] = -1;
+    if (token < T) {
+      s[i] = seq[token];
+      p[i] = pos[token];
+      if (on) v[i] = *reinterpret_cast<const h16x8*>(t.x + token * t.sx_t + g * t.sx_g + 8 * sub);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {                                             // -1: a padding row, or one the table has no page for
+    page[i] = -1;
+    if (s[i] >= 0 && s[i] < B && p[i] >= 0 && (p[i] >> log_p) < max_pages) page[i] = table[s[i] * st_b + (p[i] >> log_p)];
+    if (page[i] >= n_pages) page[i] = -1;
+  }
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    h16x2 meta;
+    const unsigned bits = quantise8(v[i], on, t.lanes, meta);
+    if (page[i] < 0) continue;
+    const int64_t slot = (((int64_t)page[i] * G + g) << log_p) + (p[i] & ((1 << log_p) - 1));
+    if (on) t.codes[slot * (t.R >> 3) + sub] = bits;
+    if (sub == 0) t.meta[slot] = __builtin_bit_cast(unsigned, meta);
+  }
 }
 
 struct CopyArrays {
@@ -147,12 +178,20 @@ extern "C" int palu_paged_append_q4(const void* k, int64_t sk_t, int64_t sk_g, c
                "paged_append: the pages must be 16-byte aligned");
   const AppendTensor a = {(const h16*)k, sk_t, sk_g, (unsigned*)k_codes, (unsigned*)k_meta, Rk, row_lanes(Rk)};
   const AppendTensor b = {(const h16*)v, sv_t, sv_g, (unsigned*)v_codes, (unsigned*)v_meta, Rv, row_lanes(Rv)};
-  const int64_t rows = (int64_t)T * G;
-  const int64_t wa = (rows + 64 / a.lanes - 1) / (64 / a.lanes), wb = (rows + 64 / b.lanes - 1) / (64 / b.lanes);
-  const int64_t wgs = (wa + wb + 3) / 4;
-  PALU_REQUIRE(wgs < (1ll << 31), PALU_ERR_ARG, "paged_append: too many rows (%lld)", (long long)rows);
-  hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream, a, b, block_table, st_b, B,
-                     max_pages, seq_ids, positions, rows, wa, G, log_p, n_pages);
+  PALU_REQUIRE(G < 65536, PALU_ERR_ARG, "paged_append: too many groups (%d)", G);
+  const int most = a.lanes > b.lanes ? a.lanes : b.lanes;
+  const int64_t waves = ((int64_t)T * most + 63) / 64;
+  // four turns a wave once that still leaves every SIMD of the device its waves
+  const bool deep = waves * 2 * G >= (int64_t)palu_num_cus() * 4 * 8 * 4;
+  const int64_t wgs = (waves + (deep ? 16 : 4) - 1) / (deep ? 16 : 4);
+  dim3 grid((unsigned)wgs, (unsigned)G, 2), block(256);
+  hipStream_t st = (hipStream_t)stream;
+  if (deep)
+    hipLaunchKernelGGL(paged_append_kernel<4>, grid, block, 0, st, a, b, block_table, st_b, B, max_pages, seq_ids, positions, T, G, log_p,
+                       n_pages);
+  else
+    hipLaunchKernelGGL(paged_append_kernel<1>, grid, block, 0, st, a, b, block_table, st_b, B, max_pages, seq_ids, positions, T, G, log_p,
+                       n_pages);
   PALU_LAUNCH_CHECK();
   return PALU_OK;
 }

@@ -18,7 +18,7 @@ Everything runs on the current stream and allocates only through torch's caching
 from __future__ import annotations
 
 import math
-from typing import NamedTuple, Optional
+from typing import Optional
 
 import torch
 
@@ -28,15 +28,48 @@ from .abx_rope import rope_inv_freq
 __all__ = ["PagePool", "make_pool", "paged_append", "paged_attn", "paged_copy", "prepare_paged_b"]
 
 
-class PagePool(NamedTuple):
-    """The four arrays of a pool: contiguous, on one GPU, [N, G, P, ...] or [layers, N, G, P, ...]."""
-    k_codes: torch.Tensor
-    k_meta: torch.Tensor
-    v_codes: torch.Tensor
-    v_meta: torch.Tensor
+class PagePool(tuple):
+    """The four arrays of a pool (k_codes, k_meta, v_codes, v_meta): contiguous, on one GPU, [N, G, P, ...] or [layers, N, G, P, ...].
+    Checked once, when it is made; a program keeps it as it keeps the arrays.  num_pages, num_groups, page_size, rank_k, rank_v (ranks
+    of one group) and layers (1 without the axis) are its sizes."""
+
+    def __new__(cls, k_codes: torch.Tensor, k_meta: torch.Tensor, v_codes: torch.Tensor, v_meta: torch.Tensor):
+        arrays = (k_codes, k_meta, v_codes, v_meta)
+        if k_codes.dim() not in (4, 5):
+            raise ValueError(f"PagePool: the arrays must be [layers,] [N, G, P, ...], got {tuple(k_codes.shape)}")
+        lead, dev = k_codes.shape[:-1], k_codes.device
+        if v_codes.shape[:-1] != lead or k_meta.shape != (*lead, 2) or v_meta.shape != (*lead, 2):
+            raise ValueError(f"PagePool: the arrays disagree: {[tuple(t.shape) for t in arrays]}")
+        if any(t.dtype != d for t, d in zip(arrays, (torch.uint8, torch.float16) * 2)):
+            raise TypeError(f"PagePool: codes are uint8 and meta fp16, got {[t.dtype for t in arrays]}")
+        if any(t.device != dev for t in arrays):
+            raise ValueError(f"PagePool: the arrays must lie on one device, got {[str(t.device) for t in arrays]}")
+        if not all(t.is_contiguous() and t.data_ptr() % 16 == 0 for t in arrays):
+            raise ValueError("PagePool: the arrays must be contiguous and 16-byte aligned")
+        self = super().__new__(cls, arrays)
+        self.layered = k_codes.dim() == 5
+        self.layers = lead[0] if self.layered else 1
+        self.num_pages, self.num_groups, self.page_size = lead[-3:]
+        self.rank_k, self.rank_v = 2 * k_codes.shape[-1], 2 * v_codes.shape[-1]
+        self.device = dev
+        if min(lead) < 1:
+            raise ValueError("PagePool: the pool is empty")
+        if self.page_size < 16 or self.page_size & (self.page_size - 1):
+            raise ValueError(f"PagePool: the page size must be a power of two >= 16, got {self.page_size}")
+        if any(r % 8 or r < 8 or r > 512 for r in (self.rank_k, self.rank_v)):
+            raise ValueError(f"PagePool: group ranks must be multiples of 8 up to 512, got {self.rank_k}, {self.rank_v}")
+        self._ptrs = tuple(t.data_ptr() for t in arrays)
+        return self
+
+    k_codes = property(lambda self: self[0])
+    k_meta = property(lambda self: self[1])
+    v_codes = property(lambda self: self[2])
+    v_meta = property(lambda self: self[3])
 
     def layer(self, i: int) -> "PagePool":
         """The pool of layer i of a pool with an axis of layers (views)."""
+        if not self.layered:
+            raise ValueError("PagePool.layer: this pool has no axis of layers")
         return PagePool(*(t[i] for t in self))
 
 
@@ -50,31 +83,25 @@ def make_pool(num_pages: int, num_groups: int, page_size: int, rank_k: int, rank
     return PagePool(t(rank_k // 2, torch.uint8), t(2, torch.float16), t(rank_v // 2, torch.uint8), t(2, torch.float16))
 
 
-def _pool_sizes(pool: PagePool, what: str, layers: bool = False):
-    """(layers, N, G, P, Rk, Rv) of a checked pool."""
-    kc, km, vc, vm = pool
-    nd = kc.dim()
-    if nd not in ((4, 5) if layers else (4,)):
-        raise ValueError(f"{what}: the pool's arrays must be [{'[layers,] ' if layers else ''}N, G, P, ...], got {tuple(kc.shape)}"
-                         + ("" if layers or nd != 5 else " (pick a layer: pool.layer(i))"))
-    lead = kc.shape[:-1]
-    if vc.shape[:-1] != lead or km.shape != (*lead, 2) or vm.shape != (*lead, 2):
-        raise ValueError(f"{what}: the pool's arrays disagree: {[tuple(t.shape) for t in pool]}")
-    if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or km.dtype != torch.float16 or vm.dtype != torch.float16:
-        raise TypeError(f"{what}: codes are uint8 and meta fp16, got {[t.dtype for t in pool]}")
-    dev = kc.device
-    for t in pool:
-        if not t.is_cuda or t.device != dev:
-            raise TypeError(f"{what}: the pool must lie on one ROCm device (no CPU fallback)")
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: the pool's arrays must be contiguous")
-    n_layers = kc.shape[0] if nd == 5 else 1
-    N, G, P = lead[-3:]
-    if N < 1 or G < 1:
-        raise ValueError(f"{what}: the pool is empty")
-    if P < 16 or P & (P - 1):
-        raise ValueError(f"{what}: the page size must be a power of two >= 16, got {P}")
-    return n_layers, N, G, P, kc.shape[-1] * 2, vc.shape[-1] * 2
+def _pool(pool: PagePool, what: str, layers: bool = False) -> PagePool:
+    if type(pool) is not PagePool:
+        raise TypeError(f"{what}: the pool must be a PagePool")
+    if not pool[0].is_cuda:
+        raise TypeError(f"{what}: the pool must lie on a ROCm device (no CPU fallback)")
+    if pool.layered and not layers:
+        raise ValueError(f"{what}: one layer at a time (pick a layer: pool.layer(i))")
+    return pool
+
+
+def _launch(dev, fn, name: str, *args):
+    """fn(*args, stream) on the current stream of `dev`, which is made the current device if it is not"""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, _lib.current_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _lib.current_stream(dev))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _int32(t: torch.Tensor, name: str, dim: int, dev, what: str) -> torch.Tensor:
@@ -94,27 +121,25 @@ def paged_append(pool: PagePool, k: torch.Tensor, v: torch.Tensor, block_table: 
     position marks a padding row and is skipped, like a row whose sequence, table entry or page does not exist.  No two rows of a
     call may name the same place."""
     what = "paged_append"
-    _, N, G, P, Rk, Rv = _pool_sizes(pool, what)
-    dev = pool.k_codes.device
+    _pool(pool, what)
+    dev, G, Rk, Rv = pool.device, pool.num_groups, pool.rank_k, pool.rank_v
     for t, name, R in ((k, "k", Rk), (v, "v", Rv)):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.device != dev:
             raise TypeError(f"{what}: {name} must be an fp16 tensor on the pool's device")
-        if t.dim() != 3 or t.shape[1:] != (G, R):
+        if t.dim() != 3 or t.shape[1] != G or t.shape[2] != R:
             raise ValueError(f"{what}: {name} must be [T, {G}, {R}], got {tuple(t.shape)}")
     T = k.shape[0]
     table = _int32(block_table, "block_table", 2, dev, what)
     seq, pos = _int32(seq_ids, "seq_ids", 1, dev, what), _int32(positions, "positions", 1, dev, what)
     if v.shape[0] != T or seq.shape[0] != T or pos.shape[0] != T:
         raise ValueError(f"{what}: k, v, seq_ids and positions must have one entry per row ({T})")
-    if T == 0 or table.shape[0] == 0 or table.shape[1] == 0:
+    B, M = table.shape
+    if T == 0 or B == 0 or M == 0:
         return
     k, v = _rows16(k), _rows16(v)
-    with _lib.on_device(k):
-        _lib.check(_lib.lib.palu_paged_append_q4(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), pool.k_codes.data_ptr(),
-            pool.k_meta.data_ptr(), pool.v_codes.data_ptr(), pool.v_meta.data_ptr(), table.data_ptr(), table.stride(0),
-            table.shape[0], table.shape[1], seq.data_ptr(), pos.data_ptr(), T, G, P, N, Rk, Rv, _lib.current_stream()),
-            "palu_paged_append_q4")
+    _launch(dev, _lib.lib.palu_paged_append_q4, "palu_paged_append_q4", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+            v.stride(0), v.stride(1), *pool._ptrs, table.data_ptr(), table.stride(0), B, M, seq.data_ptr(), pos.data_ptr(), T, G,
+            pool.page_size, pool.num_pages, Rk, Rv)
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -144,8 +169,8 @@ def paged_copy(pool: PagePool, src, dst) -> None:
     `src` and `dst`: sequences of ints (checked: pages of the pool, targets distinct and no source among them), or int32 tensors on
     the pool's device, for which the caller answers for that (a pair that names no page of the pool is skipped)."""
     what = "paged_copy"
-    layers, N, G, P, Rk, Rv = _pool_sizes(pool, what, layers=True)
-    dev = pool.k_codes.device
+    _pool(pool, what, layers=True)
+    dev, N = pool.device, pool.num_pages
     s, s_list = _page_pairs(src, "src", N, dev, what)
     d, d_list = _page_pairs(dst, "dst", N, dev, what)
     if (s_list is None) != (d_list is None):
@@ -157,16 +182,14 @@ def paged_copy(pool: PagePool, src, dst) -> None:
             raise ValueError(f"{what}: the targets must be distinct and none of them a source")
         if not s_list:
             return
-        both = torch.tensor([s_list, d_list], dtype=torch.int32).to(dev)
-        s, d = both[0], both[1]
+        s, d = torch.tensor([s_list, d_list], dtype=torch.int32).to(dev)
     elif s.shape != d.shape:
         raise ValueError(f"{what}: {s.shape[0]} sources for {d.shape[0]} targets")
-    if s.shape[0] == 0:
+    n = s.shape[0]
+    if n == 0:
         return
-    with _lib.on_device(s):
-        _lib.check(_lib.lib.palu_paged_copy(pool.k_codes.data_ptr(), pool.k_meta.data_ptr(), pool.v_codes.data_ptr(),
-                                            pool.v_meta.data_ptr(), s.data_ptr(), d.data_ptr(), s.shape[0], layers, N, G, P, Rk,
-                                            Rv, _lib.current_stream()), "palu_paged_copy")
+    _launch(dev, _lib.lib.palu_paged_copy, "palu_paged_copy", *pool._ptrs, s.data_ptr(), d.data_ptr(), n, pool.layers, N,
+            pool.num_groups, pool.page_size, pool.rank_k, pool.rank_v)
 
 
 def prepare_paged_b(b: torch.Tensor, num_groups: int) -> torch.Tensor:
@@ -181,9 +204,7 @@ def prepare_paged_b(b: torch.Tensor, num_groups: int) -> torch.Tensor:
                          f"256; got H={H}, num_groups={num_groups}, Rk={Rk}, head_dim={D}")
     b = b.contiguous()
     out = torch.empty(n, dtype=torch.uint8, device=b.device)
-    with _lib.on_device(b):
-        _lib.check(_lib.lib.palu_paged_prepare_b(b.data_ptr(), H, num_groups, Rk, D, out.data_ptr(), _lib.current_stream()),
-                   "palu_paged_prepare_b")
+    _launch(b.device, _lib.lib.palu_paged_prepare_b, "palu_paged_prepare_b", b.data_ptr(), H, num_groups, Rk, D, out.data_ptr())
     return out
 
 
@@ -199,8 +220,8 @@ def paged_attn(q: torch.Tensor, bfrag: torch.Tensor, pool: PagePool, block_table
     A sequence of length 0 gives zeros.  A length beyond the block table, or a page outside the pool within the length, gives NaN
     for that sequence; entries past the length are never read."""
     what = "paged_attn"
-    _, N, G, P, Rk, Rv = _pool_sizes(pool, what)
-    dev = pool.k_codes.device
+    _pool(pool, what)
+    dev, G, P, Rk, Rv = pool.device, pool.num_groups, pool.page_size, pool.rank_k, pool.rank_v
     if not isinstance(q, torch.Tensor) or q.dtype != torch.float16 or q.device != dev:
         raise TypeError(f"{what}: q must be an fp16 tensor on the pool's device")
     if q.dim() != 3 or q.shape[2] != 128 or q.shape[1] % G:
@@ -209,20 +230,18 @@ def paged_attn(q: torch.Tensor, bfrag: torch.Tensor, pool: PagePool, block_table
     table = _int32(block_table, "block_table", 2, dev, what)
     lens = _int32(seq_lens, "seq_lens", 1, dev, what)
     qpos = None if q_positions is None else _int32(q_positions, "q_positions", 1, dev, what)
+    M = table.shape[1]
     if table.shape[0] != B or lens.shape[0] != B or (qpos is not None and qpos.shape[0] != B):
         raise ValueError(f"{what}: block_table, seq_lens and q_positions must have one entry per query ({B})")
-    if bfrag.device != dev or bfrag.dtype != torch.uint8 or bfrag.numel() != _lib.lib.palu_paged_b_bytes(H, G, Rk) or not bfrag.numel():
+    lib = _lib.lib
+    need = lib.palu_paged_b_bytes(H, G, Rk)
+    if need == 0 or bfrag.dtype != torch.uint8 or bfrag.numel() != need or bfrag.device != dev or not bfrag.is_contiguous():
         raise ValueError(f"{what}: bfrag is not prepare_paged_b's layout of a B for H={H}, num_groups={G}, Rk={Rk} on {dev}")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = _rows16(q)
-    M = table.shape[1]
+    q = _rows16(q)
     ctx = torch.empty((B, H, Rv), dtype=torch.float16, device=dev)
-    with _lib.on_device(q):
-        ws = torch.empty(_lib.lib.palu_paged_attn_workspace_bytes(B, H, G, M, P, Rk, Rv), dtype=torch.uint8, device=dev)
-        inv = rope_inv_freq(dev, D, theta)
-        _lib.check(_lib.lib.palu_paged_attn_q4(
-            q.data_ptr(), q.stride(0), q.stride(1), bfrag.data_ptr(), pool.k_codes.data_ptr(), pool.k_meta.data_ptr(),
-            pool.v_codes.data_ptr(), pool.v_meta.data_ptr(), table.data_ptr(), table.stride(0), M, lens.data_ptr(),
-            0 if qpos is None else qpos.data_ptr(), inv.data_ptr(), ctx.data_ptr(), ws.data_ptr(), B, H, G, D, P, N, Rk, Rv,
-            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _lib.current_stream()), "palu_paged_attn_q4")
+    ws = torch.empty(lib.palu_paged_attn_workspace_bytes(B, H, G, M, P, Rk, Rv), dtype=torch.uint8, device=dev)
+    inv = rope_inv_freq(dev, D, theta)
+    _launch(dev, lib.palu_paged_attn_q4, "palu_paged_attn_q4", q.data_ptr(), q.stride(0), q.stride(1), bfrag.data_ptr(), *pool._ptrs,
+            table.data_ptr(), table.stride(0), M, lens.data_ptr(), 0 if qpos is None else qpos.data_ptr(), inv.data_ptr(),
+            ctx.data_ptr(), ws.data_ptr(), B, H, G, D, P, pool.num_pages, Rk, Rv, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale))
     return ctx
