@@ -138,11 +138,11 @@ def invalidate_b(b: torch.Tensor | None = None) -> None:
     through `.data` (`b.data.copy_(...)`, the idiom of weight loading and of fuse_hadamard) change none of them, so code
     that mutates B that way calls this afterwards (LlamaPaluAttention.fuse_hadamard / load_state_dict hooks do)."""
     if b is None:
-        _bfrag_cache.clear()
-        _shared_cache.clear()
+        for cache in (_bfrag_cache, _shared_cache, _paged_cache):
+            cache.clear()
     else:
-        _bfrag_cache.pop(id(b), None)
-        _shared_cache.pop(id(b), None)
+        for cache in (_bfrag_cache, _shared_cache, _paged_cache):
+            cache.pop(id(b), None)
 
 
 def prepare_b(b: torch.Tensor, num_groups: int) -> torch.Tensor:
@@ -171,6 +171,25 @@ def prepare_b(b: torch.Tensor, num_groups: int) -> torch.Tensor:
 
 
 _shared_cache: dict = {}
+_paged_cache: dict = {}
+
+
+def paged_b(b: torch.Tensor, num_groups: int) -> torch.Tensor:
+    """The weight B [H,R,D] in `paged_attn`'s layout (kernel/paged.py: prepare_paged_b), cached per tensor like prepare_b."""
+    hit = _paged_cache.get(id(b))
+    if hit is not None:
+        ref, ver, ptr, G, frag = hit
+        if ref() is b and ver == b._version and ptr == b.data_ptr() and G == num_groups:
+            return frag
+    from .paged import prepare_paged_b
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("paged_b: the weight's layout is made outside a graph capture (call prepare_decode(paged=True) first)")
+    frag = prepare_paged_b(b.detach(), num_groups)
+    if len(_paged_cache) > 256:
+        for k in [k for k, v in list(_paged_cache.items()) if v[0]() is None]:
+            del _paged_cache[k]
+    _paged_cache[id(b)] = (weakref.ref(b), b._version, b.data_ptr(), num_groups, frag)
+    return frag
 
 
 def shared_b(b: torch.Tensor, num_groups: int):

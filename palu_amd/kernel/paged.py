@@ -17,15 +17,18 @@ Everything runs on the current stream and allocates only through torch's caching
 """
 from __future__ import annotations
 
+import heapq
 import math
-from typing import Optional
+from numbers import Integral
+from typing import Iterable, List, Optional, Sequence, Union
 
+import numpy as np
 import torch
 
 from .. import _lib
 from .abx_rope import rope_inv_freq
 
-__all__ = ["PagePool", "make_pool", "paged_append", "paged_attn", "paged_copy", "prepare_paged_b"]
+__all__ = ["OutOfPages", "PagePool", "PagedLatentCache", "make_pool", "paged_append", "paged_attn", "paged_copy", "prepare_paged_b"]
 
 
 class PagePool(tuple):
@@ -245,3 +248,274 @@ def paged_attn(q: torch.Tensor, bfrag: torch.Tensor, pool: PagePool, block_table
             table.data_ptr(), table.stride(0), M, lens.data_ptr(), 0 if qpos is None else qpos.data_ptr(), inv.data_ptr(),
             ctx.data_ptr(), ws.data_ptr(), B, H, G, D, P, pool.num_pages, Rk, Rv, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale))
     return ctx
+
+
+class OutOfPages(RuntimeError):
+    """The pool has too few free pages for a step; nothing has changed (free a sequence, or grow the pool, and begin again)."""
+
+
+class _Sequence:
+    __slots__ = ("row", "pages", "length")
+
+    def __init__(self, max_pages: int):
+        self.row = np.full(max_pages, -1, dtype=np.int32)      # the block table's row
+        self.pages = 0                                         # pages it holds a reference to: row[:pages]
+        self.length = 0                                        # rows written
+
+
+class _Step:
+    """What the kernels of one step read: `lens` [B] with the step's rows counted, `table` [B, max_pages], and of every new row its
+    sequence (an index into the batch) and position."""
+    __slots__ = ("ids", "counts", "lens", "seq", "pos", "table")
+
+
+class PagedLatentCache:
+    """The 4-bit latents of many sequences, all layers in one pool, with the bookkeeping of a server.
+
+        cache = PagedLatentCache(layers=32, num_groups=8, rank_k=128, rank_v=384, num_pages=4096, max_seqs=64, max_pages=512)
+        a = cache.add()
+        cache.begin([a], tokens=n); ...every layer's forward on the prompt, past_key_value=cache...; cache.commit()
+        b = cache.fork(a)                                                     # shares a's pages until one of them writes
+        cache.begin([a, b]); ...every layer's forward on [2, 1, hidden]...; cache.commit()
+        cache.free(a); cache.compact()
+
+    `begin` opens a step: it reserves the pages of the new rows, copies an open page that a fork still shares (all layers and
+    sequences in one launch), and uploads the step's table, lengths and positions.  Each layer then appends its rows and attends
+    (`LlamaPaluAttention.forward` with past_key_value=cache, or `append` / `attend`), and `commit` counts the rows in.  The
+    bookkeeping lives on the host and never waits for the GPU.
+
+    The tensors of a decode step of B sequences (one token each) keep their addresses, so a graph captured inside such a step may be
+    replayed inside any later one of B sequences; `resize` moves the pool and ends that.  Work goes to the current stream: one
+    stream at a time, as for any tensor.  max_seqs bounds the sequences of one step, max_pages the pages of one sequence; rank_k / rank_v
+    are ranks of ONE group; page_size is a power of two from 16 on."""
+
+    def __init__(self, layers: int, num_groups: int, rank_k: int, rank_v: int, num_pages: int, max_seqs: int, max_pages: int,
+                 page_size: int = 64, device="cuda"):
+        if min(layers, max_seqs, max_pages) < 1:
+            raise ValueError("PagedLatentCache: layers, max_seqs and max_pages must be positive")
+        self.pool = make_pool(num_pages, num_groups, page_size, rank_k, rank_v, layers=layers, device=device)
+        self._layers = [self.pool.layer(i) for i in range(layers)]
+        self.max_seqs, self.max_pages, self.page_size = int(max_seqs), int(max_pages), int(page_size)
+        self._refs = np.zeros(num_pages, dtype=np.int64)
+        self._free: List[int] = list(range(num_pages))         # a heap: low pages first, so the pool's end stays empty longest
+        self._seqs: dict = {}
+        self._next = 0
+        self._step: Optional[_Step] = None
+        self._dev = torch.empty(self.max_seqs * (self.max_pages + 3), dtype=torch.int32, device=self.pool.device)
+
+    # -- sequences -----------------------------------------------------------------------------
+    @property
+    def num_free(self) -> int:
+        """free pages of the pool"""
+        return len(self._free)
+
+    @property
+    def sequences(self) -> list:
+        return list(self._seqs)
+
+    def __len__(self):
+        return len(self._layers)
+
+    def length(self, seq: int) -> int:
+        """committed rows of a sequence"""
+        return self._get(seq, "length").length
+
+    def pages(self, seq: int) -> list:
+        """the pages that hold a sequence's committed rows, in order"""
+        s = self._get(seq, "pages")
+        return s.row[:-(-s.length // self.page_size)].tolist()
+
+    def _get(self, seq, what: str) -> _Sequence:
+        s = self._seqs.get(seq)
+        if s is None:
+            raise KeyError(f"PagedLatentCache.{what}: there is no sequence {seq!r}")
+        return s
+
+    def _closed(self, what: str):
+        if self._step is not None:
+            raise RuntimeError(f"PagedLatentCache.{what}: a step is open (commit or abort it first)")
+
+    def _opened(self, what: str) -> _Step:
+        if self._step is None:
+            raise RuntimeError(f"PagedLatentCache.{what}: no step is open (call begin first)")
+        return self._step
+
+    def add(self) -> int:
+        """A new, empty sequence -> its id (ids are never given out twice)."""
+        seq, self._next = self._next, self._next + 1
+        self._seqs[seq] = _Sequence(self.max_pages)
+        return seq
+
+    def fork(self, seq: int) -> int:
+        """A new sequence with the same rows.  No row is copied here: the pages are shared, and the first of the two to write into
+        the open page copies that one page when its step begins."""
+        self._closed("fork")
+        s = self._get(seq, "fork")
+        new = self.add()
+        t = self._seqs[new]
+        t.pages = -(-s.length // self.page_size)
+        t.length = s.length
+        t.row[:t.pages] = s.row[:t.pages]
+        self._refs[t.row[:t.pages]] += 1
+        return new
+
+    def free(self, seq: int) -> None:
+        """End a sequence; pages that no other one shares return to the pool."""
+        self._closed("free")
+        s = self._get(seq, "free")
+        del self._seqs[seq]
+        held = s.row[:s.pages]
+        self._refs[held] -= 1
+        for p in held[self._refs[held] == 0].tolist():
+            heapq.heappush(self._free, p)
+
+    def compact(self) -> int:
+        """Move the pages in use to the front of the pool (one launch over all layers) -> their number n; pages n .. are free."""
+        self._closed("compact")
+        used = np.flatnonzero(self._refs)
+        n = len(used)
+        src = used[used >= n]
+        dst = np.flatnonzero(self._refs[:n] == 0)
+        if len(src):
+            paged_copy(self.pool, src.tolist(), dst.tolist())
+            to = np.arange(len(self._refs), dtype=np.int32)
+            to[src] = dst
+            for s in self._seqs.values():
+                s.row[:s.pages] = to[s.row[:s.pages]]
+            self._refs[dst], self._refs[src] = self._refs[src], 0
+        self._free = list(range(n, len(self._refs)))
+        return n
+
+    def resize(self, num_pages: int) -> None:
+        """A pool of num_pages pages in place of this one, with the same contents (compact first to make it smaller).  Graphs that
+        were captured over the old pool must not be replayed any more."""
+        self._closed("resize")
+        used = np.flatnonzero(self._refs)
+        least = int(used[-1]) + 1 if len(used) else 1
+        if num_pages < least:
+            raise ValueError(f"PagedLatentCache.resize: pages up to {least - 1} are in use, {num_pages} do not hold them")
+        old, keep = self.pool, min(num_pages, self.pool.num_pages)
+        new = make_pool(num_pages, old.num_groups, old.page_size, old.rank_k, old.rank_v, layers=old.layers, device=old.device)
+        for a, b in zip(new, old):
+            a[:, :keep].copy_(b[:, :keep])
+        self.pool = new
+        self._layers = [new.layer(i) for i in range(new.layers)]
+        refs = np.zeros(num_pages, dtype=np.int64)
+        refs[:keep] = self._refs[:keep]
+        self._refs = refs
+        self._free = np.flatnonzero(refs == 0).tolist()
+
+    # -- steps ---------------------------------------------------------------------------------
+    def begin(self, seqs: Iterable[int], tokens: Union[int, Sequence[int]] = 1) -> None:
+        """Open a step that writes `tokens` new rows (one number, or one per sequence) to each of the distinct sequences `seqs`."""
+        what = "begin"
+        self._closed(what)
+        ids = list(seqs)
+        counts = [int(tokens)] * len(ids) if isinstance(tokens, Integral) else [int(t) for t in tokens]
+        if not 1 <= len(ids) <= self.max_seqs or len(set(ids)) != len(ids):
+            raise ValueError(f"PagedLatentCache.begin: a step takes 1 to {self.max_seqs} distinct sequences, got {ids}")
+        if len(counts) != len(ids) or min(counts) < 1:
+            raise ValueError(f"PagedLatentCache.begin: every sequence needs at least one token, got {counts}")
+        P, M = self.page_size, self.max_pages
+        batch = [self._get(i, what) for i in ids]
+        need, shared, left = [], [], {}
+        for i, s, n in zip(ids, batch, counts):
+            if s.length + n > M * P:
+                raise ValueError(f"PagedLatentCache.begin: sequence {i} would hold {s.length + n} rows, its {M} pages hold {M * P}")
+            need.append(max(0, -(-(s.length + n) // P) - s.pages))
+            if s.length % P:                                  # of the sharers of an open page the last one keeps it
+                p = int(s.row[s.length // P])
+                left.setdefault(p, int(self._refs[p]))
+                if left[p] > 1:
+                    left[p] -= 1
+                    shared.append((s, s.length // P, p))
+        want = sum(need) + len(shared)
+        if want > len(self._free):
+            raise OutOfPages(f"PagedLatentCache.begin: the step needs {want} pages, {len(self._free)} are free")
+        fresh = [heapq.heappop(self._free) for _ in range(want)]
+        if shared:
+            try:
+                paged_copy(self.pool, [p for _, _, p in shared], fresh[:len(shared)])
+            except BaseException:
+                for p in fresh:
+                    heapq.heappush(self._free, p)
+                raise
+        self._refs[fresh] = 1
+        for (s, j, p), q in zip(shared, fresh):
+            self._refs[p] -= 1
+            s.row[j] = q
+        at = len(shared)
+        for s, n in zip(batch, need):
+            s.row[s.pages:s.pages + n] = fresh[at:at + n]
+            s.pages += n
+            at += n
+        self._step = self._upload(ids, batch, counts)
+
+    def _upload(self, ids, batch, counts) -> _Step:
+        """[lens | seq | pos | table] through one copy.  The host side is a new pinned buffer each time (torch gives its memory out
+        again only when the copy is done); the device side starts at one address, and a decode step's views depend on B alone."""
+        B, T, M = len(batch), sum(counts), self.max_pages
+        n = B + 2 * T + B * M
+        cuda = self.pool.device.type == "cuda"
+        host = torch.empty(n, dtype=torch.int32, pin_memory=cuda)
+        a = host.numpy()
+        a[:B] = [s.length + c for s, c in zip(batch, counts)]
+        a[B:B + T] = np.repeat(np.arange(B), counts)
+        a[B + T:B + 2 * T] = np.concatenate([np.arange(s.length, s.length + c) for s, c in zip(batch, counts)])
+        for i, s in enumerate(batch):
+            a[B + 2 * T + i * M:B + 2 * T + (i + 1) * M] = s.row
+        dev = self._dev[:n] if n <= self._dev.numel() else torch.empty(n, dtype=torch.int32, device=self.pool.device)
+        dev.copy_(host, non_blocking=cuda)
+        step = _Step()
+        step.ids, step.counts = ids, counts
+        step.lens, step.seq, step.pos, step.table = dev.split([B, T, T, B * M])
+        step.table = step.table.view(B, M)
+        return step
+
+    def commit(self) -> None:
+        """Close the step: its rows are part of their sequences."""
+        step = self._opened("commit")
+        for i, n in zip(step.ids, step.counts):
+            self._seqs[i].length += n
+        self._step = None
+
+    def abort(self) -> None:
+        """Close the step without its rows (pages it reserved stay with their sequences and serve the next step)."""
+        self._opened("abort")
+        self._step = None
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Write the step's rows of one layer: k [T, G, Rk], v [T, G, Rv] fp16, the sequences' rows one after another."""
+        step = self._opened("append")
+        paged_append(self._layers[layer], k, v, step.table, step.seq, step.pos)
+
+    def adopt(self, layer: int, rows, index: int = 0) -> None:
+        """Take one layer's packed rows from a QuantLatentCache (4 bit, one scale a row) as the rows of the step's sequence number
+        `index`, which must be empty: how a prompt pass hands its cache over.  The codes move as they are."""
+        step = self._opened("adopt")
+        seq, n, pool = step.ids[index], step.counts[index], self._layers[layer]
+        if self._seqs[seq].length:
+            raise ValueError(f"PagedLatentCache.adopt: sequence {seq} is not empty")
+        if rows.n_bits != 4 or rows.group_size or rows.get_seq_length(layer) != n:
+            raise ValueError(f"PagedLatentCache.adopt: need {n} rows of 4 bits with one scale a row, got {rows.get_seq_length(layer)} "
+                             f"rows of {rows.n_bits} bits, group_size {rows.group_size}")
+        st = rows.buffers(layer)
+        if (st["Rk"], st["Rv"], st["kc"].shape[1]) != (pool.rank_k, pool.rank_v, pool.num_groups):
+            raise ValueError("PagedLatentCache.adopt: the ranks or groups differ from the pool's")
+        m = -(-n // self.page_size)
+        pages = step.table[index, :m].long()
+        for to, src in zip(pool, (st["kc"], st["km"], st["vc"], st["vm"])):
+            G, W = src.shape[1], src.shape[3]
+            tile = torch.zeros((G, m * self.page_size, W), dtype=src.dtype, device=src.device)
+            tile[:, :n].copy_(src[0, :, :n])
+            to.index_copy_(0, pages, tile.view(G, m, self.page_size, W).transpose(0, 1))
+
+    def attend(self, layer: int, q: torch.Tensor, bfrag: torch.Tensor, q_positions: Optional[torch.Tensor] = None,
+               theta: float = 10000.0, sm_scale: Optional[float] = None) -> torch.Tensor:
+        """The step's new tokens, one of each sequence, against the rows of one layer (append first): q [B, H, 128] fp16, not rotated
+        -> ctx [B, H, Rv].  q_positions (int32 [B]) defaults to the rows the tokens were written to."""
+        step = self._opened("attend")
+        if max(step.counts) != 1:
+            raise ValueError(f"PagedLatentCache.attend: one token of each sequence, this step writes {step.counts}")
+        return paged_attn(q, bfrag, self._layers[layer], step.table, step.lens, step.pos if q_positions is None else q_positions,
+                          theta, sm_scale)

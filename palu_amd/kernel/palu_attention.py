@@ -28,9 +28,10 @@ from torch import nn
 
 from .. import _lib
 from .abx_rope import abx as recompute_k_gemv  # same alias as kernel/palu_attention.py:13
-from .abx_rope import invalidate_b, prepare_b, rope_cs_table, rope_inv_freq, shared_b
+from .abx_rope import invalidate_b, paged_b, prepare_b, rope_cs_table, rope_inv_freq, shared_b
+from .paged import PagedLatentCache
 
-__all__ = ["HeadwiseLowRankModule", "LlamaPaluAttention", "LatentCache", "QuantLatentCache", "DynamicCache",
+__all__ = ["HeadwiseLowRankModule", "LlamaPaluAttention", "LatentCache", "QuantLatentCache", "PagedLatentCache", "DynamicCache",
            "build_b", "fuse_wo"]
 
 
@@ -1125,16 +1126,20 @@ class LlamaPaluAttention(nn.Module):
             self.o_proj.weight.data = apply_hadamard(w.reshape(w.shape[0], self.num_heads, Rv).contiguous()).reshape(w.shape)
         return self
 
-    def prepare_decode(self):
+    def prepare_decode(self, paged: bool = False):
         """Build what the HIP decode step derives from the weights -- the MFMA fragments of B and the "do the heads of a
         group share B" decision (one device comparison = one host sync) -- NOW, i.e. outside any stream capture and off
         the first token's path.  Idempotent and cached per weight tensor; call it after the module sits on its GPU and
         again after its weights changed (`fuse_hadamard` and `load_state_dict` invalidate the cache themselves).  Without
-        it the first decode step does the same lazily (which raises inside a hipGraph capture: warm up or call this first)."""
+        it the first decode step does the same lazily (which raises inside a hipGraph capture: warm up or call this first).
+        paged: for decoding on a PagedLatentCache, whose kernels read B in a layout of their own."""
         if hasattr(self.k_proj, "B") and self.k_proj.B.is_cuda:
             with _lib.on_device(self.k_proj.B):
-                bg = shared_b(self.k_proj.B, self.num_groups)
-                prepare_b(self.k_proj.B if bg is None else bg, self.num_groups)
+                if paged:
+                    paged_b(self.k_proj.B, self.num_groups)
+                else:
+                    bg = shared_b(self.k_proj.B, self.num_groups)
+                    prepare_b(self.k_proj.B if bg is None else bg, self.num_groups)
                 rope_inv_freq(self.k_proj.B.device, self.head_dim, self.rope_theta)
         return self
 
@@ -1154,6 +1159,57 @@ class LlamaPaluAttention(nn.Module):
                     and _q_scratch_ok(self, Rk) and self.num_groups * Rv <= 16384)
         return gs in (1, 2, 3, 4, 8) and Rk % 8 == 0 and Rv % 8 == 0 and Rv // 8 <= 256
 
+    # -- many sequences on pages -----------------------------------------------------------------
+    def _forward_paged(self, hidden_states, attention_mask, position_ids, cache: "PagedLatentCache", output_attentions, **kwargs):
+        """The step that is open in `cache` (its sequences are the batch): one token of each (paged_append + paged_attn), or whole
+        prompts of empty sequences (each through a packed 4-bit cache of its own, whose rows the pages then take over)."""
+        step = cache._opened("forward")
+        bsz, q_len, _ = hidden_states.shape
+        H, G, D = self.num_heads, self.num_groups, self.head_dim
+        if self.layer_idx is None:
+            raise ValueError(f"{self.__class__.__name__} on a PagedLatentCache needs a layer index")
+        if bsz != len(step.ids) or any(n != q_len for n in step.counts):
+            raise ValueError(f"hidden_states hold {q_len} tokens of {bsz} sequences, the open step takes {step.counts}")
+        if output_attentions:
+            raise NotImplementedError("a PagedLatentCache gives no attention weights")
+        if not (hidden_states.is_cuda and hidden_states.dtype == torch.float16 and D == 128 and hasattr(self.k_proj, "B")
+                and self.o_proj.in_features == self.fused_hidden_dim_o):
+            raise NotImplementedError("a PagedLatentCache serves fp16 modules of head_dim 128 on a GPU, with B and the fused o_proj")
+        if q_len == 1:
+            if attention_mask is not None:
+                raise ValueError("decoding on a PagedLatentCache takes no attention mask: every sequence attends to all of its rows")
+            if position_ids is not None:
+                position_ids = position_ids.to(device=hidden_states.device, dtype=torch.int32).reshape(-1)
+                if position_ids.numel() == 1 and bsz > 1:
+                    position_ids = position_ids.expand(bsz).contiguous()
+            frag = paged_b(self.k_proj.B, G)
+            q = self.q_proj(hidden_states).view(bsz, H, D)
+            cache.append(self.layer_idx, self.k_proj.VT(hidden_states).view(bsz, G, self.group_rank_k),
+                         self.v_proj.VT(hidden_states).view(bsz, G, self.group_rank_v))
+            ctx = cache.attend(self.layer_idx, q, frag, position_ids, self.rope_theta)
+            return self.o_proj(ctx.view(bsz, 1, -1)), None, cache
+        if any(cache.length(i) for i in step.ids):
+            raise NotImplementedError("a prompt on a PagedLatentCache starts an empty sequence (continue one token by token)")
+        # later tokens attend to every row of their sequence, rotated at its index: a prompt with another mask or other
+        # positions would be continued as something else
+        std = torch.arange(q_len, device=hidden_states.device)
+        if position_ids is not None and not bool((position_ids.to(std.device).reshape(-1, q_len) == std).all()):
+            raise ValueError("a prompt on a PagedLatentCache stands at positions 0 ..")
+        if attention_mask is not None:
+            attention_mask = additive_mask(attention_mask, hidden_states.dtype)
+            if attention_mask.shape[1:] != (1, q_len, q_len) or attention_mask.shape[0] not in (1, bsz):
+                raise ValueError(f"Attention mask should be of size {(bsz, 1, q_len, q_len)}, but is {attention_mask.size()}")
+            if not all(self._mask_is_causal(m, q_len, 0) for m in attention_mask):
+                raise ValueError("a prompt on a PagedLatentCache takes the causal mask only (no padding: one step per length)")
+            kwargs["is_causal"] = True
+        outs = []
+        for i in range(bsz):
+            rows = QuantLatentCache(4, capacity=q_len)
+            m = None if attention_mask is None else attention_mask[min(i, attention_mask.shape[0] - 1)][None]
+            outs.append(self._forward(hidden_states[i:i + 1], m, std[None], rows, False, **kwargs)[0])
+            cache.adopt(self.layer_idx, rows, i)
+        return torch.cat(outs) if bsz > 1 else outs[0], None, cache
+
     # -- forward -----------------------------------------------------------------------------
     def forward(self, hidden_states: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                 position_ids: Optional[torch.LongTensor] = None, past_key_value=None,
@@ -1171,6 +1227,8 @@ class LlamaPaluAttention(nn.Module):
                  output_attentions=False, golden_kernel=False, **kwargs):
         if "padding_mask" in kwargs:
             warnings.warn("Passing `padding_mask` is deprecated; use `attention_mask` instead.")
+        if isinstance(past_key_value, PagedLatentCache):
+            return self._forward_paged(hidden_states, attention_mask, position_ids, past_key_value, output_attentions, **kwargs)
         bsz, q_len, _ = hidden_states.size()
         H, G, D = self.num_heads, self.num_groups, self.head_dim
         if past_key_value is not None and self.layer_idx is None:

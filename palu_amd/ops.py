@@ -15,6 +15,9 @@ dispatcher (torch.compile / export see opaque ops with fake kernels).  Importing
     palu::decode_attn(q, bfrag, k, v, inv_freq, workspace!, H, L, pos0) -> Tensor  single-kernel scores+softmax+P.V
     palu::lowrank_project_gemm(x, w, cache!, row0) -> ()              prefill down-projection into the cache rows
     palu::pack_codes(codes, bits) / palu::unpack_codes(packed, bits, rank)
+    palu::paged_append(k_codes!, k_meta!, v_codes!, v_meta!, k, v, block_table, seq_ids, positions) -> ()
+    palu::paged_copy(k_codes!, k_meta!, v_codes!, v_meta!, src, dst) -> ()            pages of many sequences (kernel/paged.py)
+    palu::paged_attn(q, bfrag, k_codes, k_meta, v_codes, v_meta, block_table, seq_lens, q_positions=None, theta=1e4) -> Tensor
 
 All run on the current stream and allocate only through torch's caching allocator (graph-capturable).
 """
@@ -28,6 +31,7 @@ import torch
 from . import _lib
 from .kernel import abx_rope as _abx
 from .kernel import hadamard_utils as _had
+from .kernel import paged as _paged
 from .kernel import quant as _quant
 
 
@@ -297,3 +301,41 @@ def decode_attn(q: torch.Tensor, bfrag: torch.Tensor, k: torch.Tensor, v: torch.
 @decode_attn.register_fake
 def _(q, bfrag, k, v, inv_freq, workspace, num_heads, length, pos0=0, mask=None):
     return q.new_empty((num_heads, v.shape[2]))
+
+
+@torch.library.custom_op("palu::paged_append", mutates_args=("k_codes", "k_meta", "v_codes", "v_meta"))
+def paged_append(k_codes: torch.Tensor, k_meta: torch.Tensor, v_codes: torch.Tensor, v_meta: torch.Tensor, k: torch.Tensor,
+                 v: torch.Tensor, block_table: torch.Tensor, seq_ids: torch.Tensor, positions: torch.Tensor) -> None:
+    """Quantise rows of many sequences into their pages (kernel/paged.py: paged_append) of one layer's pool."""
+    _paged.paged_append(_paged.PagePool(k_codes, k_meta, v_codes, v_meta), k, v, block_table, seq_ids, positions)
+
+
+@paged_append.register_fake
+def _(k_codes, k_meta, v_codes, v_meta, k, v, block_table, seq_ids, positions):
+    return None
+
+
+@torch.library.custom_op("palu::paged_copy", mutates_args=("k_codes", "k_meta", "v_codes", "v_meta"))
+def paged_copy(k_codes: torch.Tensor, k_meta: torch.Tensor, v_codes: torch.Tensor, v_meta: torch.Tensor, src: torch.Tensor,
+               dst: torch.Tensor) -> None:
+    """Page dst[i] becomes a copy of page src[i] in every layer of the pool (kernel/paged.py: paged_copy)."""
+    _paged.paged_copy(_paged.PagePool(k_codes, k_meta, v_codes, v_meta), src, dst)
+
+
+@paged_copy.register_fake
+def _(k_codes, k_meta, v_codes, v_meta, src, dst):
+    return None
+
+
+@torch.library.custom_op("palu::paged_attn", mutates_args=())
+def paged_attn(q: torch.Tensor, bfrag: torch.Tensor, k_codes: torch.Tensor, k_meta: torch.Tensor, v_codes: torch.Tensor,
+               v_meta: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, q_positions: Optional[torch.Tensor] = None,
+               theta: float = 10000.0, sm_scale: Optional[float] = None) -> torch.Tensor:
+    """One new token of each of B sequences against its 4-bit pages (kernel/paged.py: paged_attn); bfrag = prepare_paged_b(B, G)."""
+    return _paged.paged_attn(q, bfrag, _paged.PagePool(k_codes, k_meta, v_codes, v_meta), block_table, seq_lens, q_positions, theta,
+                             sm_scale)
+
+
+@paged_attn.register_fake
+def _(q, bfrag, k_codes, k_meta, v_codes, v_meta, block_table, seq_lens, q_positions=None, theta=10000.0, sm_scale=None):
+    return q.new_empty((q.shape[0], q.shape[1], 2 * v_codes.shape[-1]))
