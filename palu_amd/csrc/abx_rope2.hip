@@ -182,6 +182,15 @@ extern "C" int palu_rope_table_unregister(const float* inv_freq) {
   return PALU_OK;
 }
 
+// inv_freq[32] of a registered table, 0 for another one (the paged attention's choice of its two-band form)
+float palu_rope_low_frequency(const float* inv_freq) {
+  if (!two_band_enabled()) return 0.f;
+  std::lock_guard<std::mutex> lk(g_tab_mutex);
+  for (const auto& t : g_tabs)
+    if (t.inv_freq == inv_freq) return t.f_low;
+  return 0.f;
+}
+
 // 1 when a launch with these positions would take the two-band kernel (introspection for tests and the bench)
 extern "C" int palu_abx_two_band_selected(const float* inv_freq, int H, int G, int L, int R, int pos0) {
   if (!two_band_enabled() || !palu_abx2_frag_bytes(H, G, R) || L <= 0 || pos0 < 0 || pos0 % TL) return 0;

@@ -2,72 +2,100 @@
 // of a sequence.  The attention itself is paged_attn_kernel.h.
 #include "paged_attn_kernel.h"
 
+float palu_rope_low_frequency(const float* inv_freq);      // inv_freq[32] of a registered table, else 0
+
 int palu_paged_attn_launch_lo(const void* params, int nks, int chunks, int heads, int wgs, hipStream_t stream);
 int palu_paged_attn_launch_mid(const void* params, int nks, int chunks, int heads, int wgs, hipStream_t stream);
 int palu_paged_attn_launch_hi(const void* params, int nks, int chunks, int heads, int wgs, hipStream_t stream);
 
 namespace {
 
-// Joins the pieces of one (sequence, head): 64 columns a workgroup, the pieces dealt over four waves.  Sequences that one
-// workgroup had whole are done already; empty ones get their zeros here.
-static __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnParams p, int W) {
-  __shared__ float sh[4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int GV = p.G * p.VG;
-  const int bg = blockIdx.x, b = bg / GV, gv = bg - b * GV, g = gv / p.VG, vg = gv - g * p.VG;
-  const int j = blockIdx.y, nh = min(p.heads, p.gs - p.heads * vg);
-  const int c = blockIdx.z * 64 + lane;
-  if (j >= nh) return;
-  h16* out = p.ctx + ((int64_t)b * p.H + g * p.gs + p.heads * vg + j) * p.Rv;
-  const int nt = pa_tiles(p, b);
-  if (nt == 0) {
-    if (w == 0 && c < p.Rv) out[c] = (h16)(pa_bad_len(p, b) ? NAN : 0.f);
+// Joins the pieces of one (sequence, set of heads): four columns of one head a thread; the values of the first pieces, most often all,
+// are requested together with the pieces' statistics.  Sequences that one workgroup had whole are done already; empty ones get their
+// zeros here.
+static __global__ __launch_bounds__(128) void paged_attn_join_kernel(PagedAttnParams p) {
+  const int GV = p.G * p.VG, bg = blockIdx.x, b = bg / GV, gv = bg - b * GV, g = gv / p.VG, vg = gv - g * p.VG;
+  const int per = p.Rv >> 2, item = blockIdx.y * 128 + threadIdx.x, j = item / per, c = 4 * (item - j * per);
+  if (j >= min(p.heads, p.gs - p.heads * vg)) return;
+  h16x4* const out = reinterpret_cast<h16x4*>(p.ctx + ((int64_t)b * p.H + g * p.gs + p.heads * vg + j) * p.Rv + c);
+  const int2 pc = p.pieces[bg];
+  const bool bad = pa_bad_len(p, b);
+  if (pa_tiles(p, b) == 0) {
+    const h16 v = (h16)(bad ? NAN : 0.f);
+    *out = h16x4{v, v, v, v};
     return;
   }
-  const PaLine line = pa_line(p, lane, b);
-  const int chunk = pa_chunk(p, line.total, W);
-  const int begin = line.front + gv * (nt + PA_FIX);       // the tiles lie at begin + PA_FIX .. begin + PA_FIX + nt - 1
-  const int first = (begin + PA_FIX) / chunk, last = (begin + PA_FIX + nt - 1) / chunk;
-  const int np = last - first + 1;
+  const int np = pc.y;
   if (np == 1) return;
-  const float* stat = p.part + ((int64_t)(first + bg) * 4 + j) * 2;
-  const float* val = p.part + (int64_t)p.slots * 8 + ((int64_t)(first + bg) * 4 + j) * p.Rv;
-  float top = -INFINITY;
-  for (int i = lane; i < np; i += 64) top = fmaxf(top, stat[(int64_t)i * 8]);
-  top = wave_max(top);
+  typedef float pair __attribute__((ext_vector_type(2)));
+  const int64_t at = ((int64_t)(pc.x + bg) * 4 + j);
+  const pair* stat = reinterpret_cast<const pair*>(p.part) + at;             // (maximum, sum), of the next piece 4 further
+  const float* val = p.part + (int64_t)p.slots * 8 + at * p.Rv + c;          // of the next piece 4 Rv further
+  constexpr int K = 4;
+  f32x4 v[K];
+  pair s[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int k = min(i, np - 1);
+    s[i] = stat[4 * k];
+    v[i] = *reinterpret_cast<const f32x4*>(val + (int64_t)k * 4 * p.Rv);
+  }
+  float top = fmaxf(fmaxf(s[0][0], s[1][0]), fmaxf(s[2][0], s[3][0]));
+  for (int i = K; i < np; ++i) top = fmaxf(top, stat[4 * i][0]);
   const float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
-  for (int i = lane; i < np; i += 64) sum += __builtin_amdgcn_exp2f(stat[(int64_t)i * 8] - ref) * stat[(int64_t)i * 8 + 1];
-  sum = wave_sum(sum);
-  float v = 0.f;
-  if (c < p.Rv)
-    for (int i = w; i < np; i += 4) v = fmaf(__builtin_amdgcn_exp2f(stat[(int64_t)i * 8] - ref), val[(int64_t)i * 4 * p.Rv + c], v);
-  sh[w][lane] = v;
-  __syncthreads();
-  if (w == 0 && c < p.Rv) out[c] = (h16)(pa_bad_len(p, b) ? NAN : (sh[0][lane] + sh[1][lane] + sh[2][lane] + sh[3][lane]) / sum);
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const float f = i < np ? __builtin_amdgcn_exp2f(s[i][0] - ref) : 0.f;
+    if (i < np) {                                          // (a repeated piece may hold NaN: it is not multiplied by 0)
+      sum = fmaf(f, s[i][1], sum);
+      acc += v[i] * f;
+    }
+  }
+#pragma unroll 4
+  for (int i = K; i < np; ++i) {
+    const pair st = stat[4 * i];
+    const float f = __builtin_amdgcn_exp2f(st[0] - ref);
+    sum = fmaf(f, st[1], sum);
+    acc += *reinterpret_cast<const f32x4*>(val + (int64_t)i * 4 * p.Rv) * f;
+  }
+  const float f = bad ? NAN : 1.f / sum;
+  *out = h16x4{(h16)(acc[0] * f), (h16)(acc[1] * f), (h16)(acc[2] * f), (h16)(acc[3] * f)};
 }
 
 
 // One 16-byte piece a thread: eight values of r of one column of B, in the order in which the kernel finds a word's codes.
+// Behind the pieces of the one-band form (`full` of them) follow those of the two-band form: a wave's high band, row n = head n / 8,
+// pair 4 w + 2 ((n >> 2) & 1) + ((n & 3) >> 1), cos or sin; then its low band, piece (16 columns, half of the 64 (pair, cos or sin)),
+// lane = column, four pairs of (B[r, i], B[r, i + 64]).
 __global__ __launch_bounds__(256) void paged_prepare_b_kernel(const h16* __restrict__ b, int G, int gs, int VG, int heads, int R, int nks,
-                                                              u32x4* __restrict__ out, int64_t pieces) {
+                                                              u32x4* __restrict__ out, int64_t full, int64_t pieces) {
   const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (idx >= pieces) return;
-  const int lane = (int)(idx & 63), kb = (int)((idx >> 6) % nks);
-  const int64_t rest = (idx >> 6) / nks;
-  const int mbs = heads / 2, mb = (int)(rest % mbs), w = (int)((rest / mbs) & 7), gv = (int)(rest / mbs >> 3);
-  const int n = lane & 31, e = n & 3;
-  const int g = gv / VG, hl = heads * (gv - g * VG) + 2 * mb + (n >> 4);
-  const int col = 8 * w + 4 * ((n >> 3) & 1) + 2 * ((n >> 2) & 1) + (e >> 1) + 64 * (e & 1);
-  h16x8 v;
+  const bool band = idx >= full;
+  const int64_t unit = (band ? idx - full : idx) >> 6;
+  const int lane = (int)(idx & 63);
+  const int mbs = heads / 2, piece = (int)(unit % (mbs * nks)), w = (int)(unit / (mbs * nks)) & 7, gv = (int)(unit / (mbs * nks) >> 3);
+  const int g = gv / VG, set = heads * (gv - g * VG);
   // 16-byte piece u of a position's row in LDS is word i of part `part` of the row; the last parts are moved back to end with the row,
-  // and what they then hold a second time counts for nothing
-  const int u = 2 * kb + (lane >> 5), ul = nks / 2, part = u / ul, i = u % ul;
-  const int word = min(part * ul, R / 8 - ul) + i;
-#pragma unroll
-  for (int d = 0; d < 8; ++d) {
+  // and what they then hold a second time counts for nothing.  -> B[head, r, col] of element d of piece u
+  auto value = [&](int head, int u, int d, int col) -> h16 {
+    const int ul = nks / 2, part = u / ul, word = min(part * ul, R / 8 - ul) + u % ul;
     const int r = 8 * word + (d >> 1) + 4 * (d & 1);
-    v[d] = hl < gs && word >= part * ul ? b[((int64_t)(g * gs + hl) * R + r) * 128 + col] : (h16)0.f;
+    return head < gs && word >= part * ul ? b[((int64_t)(g * gs + head) * R + r) * 128 + col] : (h16)0.f;
+  };
+  h16x8 v;
+  if (band && piece >= nks) {
+    const int i = piece - nks, rx = 16 * ((w & 1) * (nks / 2) + i / 2) + (lane & 15), pair = 32 + 16 * (i & 1) + 4 * (lane >> 4);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) v[d] = value(set + (w >> 1), rx >> 3, rx & 7, pair + (d >> 1) + 64 * (d & 1));
+  } else {
+    const int n = lane & 31, kb = piece % nks, mb = piece / nks, e = n & 3;
+    const int head = set + (band ? n >> 3 : 2 * mb + (n >> 4));
+    const int pair = (band ? 4 * w : 8 * w + 4 * ((n >> 3) & 1)) + 2 * ((n >> 2) & 1) + (e >> 1);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) v[d] = value(head, 2 * kb + (lane >> 5), d, pair + 64 * (e & 1));
   }
   out[idx] = __builtin_bit_cast(u32x4, v);
 }
@@ -81,6 +109,8 @@ int pa_nks(int R) {
 bool pa_heads_ok(int H, int G, int R) { return H > 0 && G > 0 && H % G == 0 && R > 0 && R % 8 == 0 && R <= 256; }
 // heads of a set (see paged_attn_kernel.h), and the sets of a latent group
 int pa_heads(int H, int G, int R) { return H / G <= 2 || R > 128 ? 2 : 4; }
+// the two-band form exists where 32 rows of a matrix block are four heads: its part of the fragments is as large as the other's
+bool pa_has_band(int H, int G, int R) { return pa_heads(H, G, R) == 4; }
 int pa_vg(int H, int G, int R) { return (H / G + pa_heads(H, G, R) - 1) / pa_heads(H, G, R); }
 
 struct PaPlan {
@@ -107,8 +137,10 @@ PaPlan pa_plan(int B, int H, int G, int max_pages, int P, int Rk) {
 
 }  // namespace
 
+static int64_t pa_full_pieces(int H, int G, int R) { return (int64_t)G * pa_vg(H, G, R) * 8 * (pa_heads(H, G, R) / 2) * pa_nks(R) * 64; }
+
 extern "C" size_t palu_paged_b_bytes(int H, int G, int R) {
-  return pa_heads_ok(H, G, R) ? (size_t)G * pa_vg(H, G, R) * 8 * (pa_heads(H, G, R) / 2) * pa_nks(R) * 1024 : 0;
+  return pa_heads_ok(H, G, R) ? (size_t)pa_full_pieces(H, G, R) * 16 * (pa_has_band(H, G, R) ? 2 : 1) : 0;
 }
 
 extern "C" int palu_paged_prepare_b(const void* b, int H, int G, int R, int D, void* out, palu_stream_t stream) {
@@ -118,7 +150,7 @@ extern "C" int palu_paged_prepare_b(const void* b, int H, int G, int R, int D, v
   PALU_REQUIRE(b && out && ((uintptr_t)out & 15) == 0, PALU_ERR_ARG, "paged_prepare_b: null or unaligned pointer");
   const int64_t pieces = (int64_t)palu_paged_b_bytes(H, G, R) / 16;
   hipLaunchKernelGGL(paged_prepare_b_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream, (const h16*)b, G,
-                     H / G, pa_vg(H, G, R), pa_heads(H, G, R), R, pa_nks(R), (u32x4*)out, pieces);
+                     H / G, pa_vg(H, G, R), pa_heads(H, G, R), R, pa_nks(R), (u32x4*)out, pa_full_pieces(H, G, R), pieces);
   PALU_LAUNCH_CHECK();
   return PALU_OK;
 }
@@ -126,7 +158,7 @@ extern "C" int palu_paged_prepare_b(const void* b, int H, int G, int R, int D, v
 extern "C" size_t palu_paged_attn_workspace_bytes(int B, int H, int G, int max_pages, int P, int Rk, int Rv) {
   if (B <= 0 || !pa_heads_ok(H, G, Rk) || max_pages <= 0 || P <= 0 || Rv <= 0) return 16;
   const PaPlan s = pa_plan(B, H, G, max_pages, P, Rk);
-  return s.direct ? 16 : (size_t)s.slots * (8 + 4 * (size_t)Rv) * 4;
+  return s.direct ? 16 : (size_t)s.slots * (8 + 4 * (size_t)Rv) * 4 + (size_t)B * G * pa_vg(H, G, Rk) * 8;
 }
 
 extern "C" int palu_paged_attn_q4(const void* q, int64_t sq_b, int64_t sq_h, const void* bfrag, const void* k_codes,
@@ -154,9 +186,13 @@ extern "C" int palu_paged_attn_q4(const void* q, int64_t sq_b, int64_t sq_h, con
   const int VG = pa_vg(H, G, Rk), nks = pa_nks(Rk);
   const PaPlan s = pa_plan(B, H, G, max_pages, P, Rk);
   const int heads = pa_heads(H, G, Rk);
-  const PagedAttnParams p = {(const h16*)q, sq_b, sq_h, (const h16*)bfrag, (const unsigned*)k_codes, (const unsigned*)k_meta,
+  // two bands: 64 f_32 <= 0.7 rad keeps the degree-7 polynomials of the low pairs within 0.7^8 / 8! = 1.4e-6 (theta >= ~8400)
+  const float f32 = pa_has_band(H, G, Rk) ? palu_rope_low_frequency(inv_freq) : 0.f;
+  const int band = f32 > 0.f && 64.f * f32 <= 0.7f;
+  const PagedAttnParams p = {(const h16*)q, sq_b, sq_h, (const h16*)bfrag, pa_full_pieces(H, G, Rk), (const unsigned*)k_codes, (const unsigned*)k_meta,
                              (const unsigned*)v_codes, (const unsigned*)v_meta, block_table, st_b, seq_lens, q_positions, inv_freq,
-                             (h16*)ctx, (float*)workspace, s.slots, B, H, G, H / G, VG, max_pages, log_p, n_pages, Rk, Rv, heads,
+                             (h16*)ctx, (float*)workspace, s.slots,
+                             (int2*)((float*)workspace + (int64_t)s.slots * (8 + 4 * (int64_t)Rv)), B, H, G, H / G, VG, max_pages, log_p, n_pages, Rk, Rv, heads, band,
                              s.min_chunk, s.direct, sm_scale * 1.44269504088896f};
   const int chunks = (Rv + 127) / 128;
   hipStream_t st = (hipStream_t)stream;
@@ -164,8 +200,7 @@ extern "C" int palu_paged_attn_q4(const void* q, int64_t sq_b, int64_t sq_h, con
                  : nks <= 8 ? palu_paged_attn_launch_mid(&p, nks, chunks, heads, s.wgs, st)
                             : palu_paged_attn_launch_hi(&p, nks, chunks, heads, s.wgs, st);
   if (rc != PALU_OK || s.direct) return rc;
-  hipLaunchKernelGGL(paged_attn_join_kernel, dim3((unsigned)(B * G * VG), (unsigned)heads, (unsigned)((Rv + 63) / 64)), dim3(256), 0, st, p,
-                     s.wgs);
+  hipLaunchKernelGGL(paged_attn_join_kernel, dim3((unsigned)(B * G * VG), (unsigned)((heads * Rv / 4 + 127) / 128)), dim3(128), 0, st, p);
   PALU_LAUNCH_CHECK();
   return PALU_OK;
 }

@@ -36,7 +36,8 @@ constexpr int PA_TILE = 128;             // positions of a tile
 
 struct PagedAttnParams {
   const h16* q;       int64_t sq_b, sq_h;
-  const h16* bfrag;                      // palu_paged_prepare_b's layout
+  const h16* bfrag;                      // palu_paged_prepare_b's layout, and where in it (16-byte pieces) the two-band form's part begins
+  int64_t band_at;
   const unsigned* kc; const unsigned* km;
   const unsigned* vc; const unsigned* vm;
   const int* table;   int64_t st_b;
@@ -46,9 +47,10 @@ struct PagedAttnParams {
   h16* ctx;
   float* part;                           // partial results: [slots][4][2] (maximum, sum), then [slots][4][Rv]
   int slots;
+  int2* pieces;                          // [B][G VG]: the first of a (sequence, heads)'s pieces, and how many there are
   int B, H, G, gs, VG;                   // gs = H / G heads of a latent group, dealt into VG sets of `heads` (2 or 4)
   int max_pages, log_p, n_pages, Rk, Rv;
-  int heads;
+  int heads, band;
   int min_chunk;                         // tiles a workgroup takes at least
   int direct;                            // one workgroup per (sequence, heads): no partial results, no second kernel
   float scale;                           // sm_scale log2(e)
@@ -127,6 +129,10 @@ static __device__ __forceinline__ float lane_value(float v, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
+// (A pointer that went through pa_opaque no longer shows what it points to: without the address space hipcc loads through the flat
+// path, whose loads also count as LDS accesses, and every LDS read then waits for all of them.)
+typedef const __attribute__((address_space(1))) unsigned* global_words;
+
 // N consecutive words alike, as few wide loads (a word's alignment is enough for them)
 template <int N>
 static __device__ __forceinline__ void lane_words(unsigned* out, const unsigned* row, unsigned bytes) {
@@ -151,24 +157,30 @@ static __device__ __forceinline__ int pa_query_exponent(const h16* q, int64_t sq
   return big > 0.f && big < INFINITY ? (int)(__builtin_bit_cast(unsigned, big) >> 23) - 131 : 0;
 }
 
-template <int NKS, int NH>
+template <int NKS, int NH, bool BAND>
 struct PaLds {
   static constexpr int XS = NKS * 32 + 16;                 // bytes of a position's row: 16 more, so that 8 lanes reading 16 bytes of 8 rows meet 8 bank groups
-  static constexpr int RED = 2 * PA_TILE * XS;             // float [2][8 waves][NH heads][PA_TILE]
-  static constexpr int WGT = RED + 2 * 8 * NH * PA_TILE * 4;   // h16 [4 waves]: weights [4 heads][32], zeros [32]
+  static constexpr int NP = BAND ? 10 : 8;                 // partial scores of a position: of eight waves, and two of the low band
+  static constexpr int RED = 2 * PA_TILE * XS;             // float [2][NP][NH heads][PA_TILE]
+  static constexpr int WGT = RED + 2 * NP * NH * PA_TILE * 4;  // h16 [4 waves]: weights [4 heads][32], zeros [32]
   static constexpr int STEP = WGT + 4 * 160 * 2;           // f32x4 [8 waves][2 halves][2]: cos / sin of a 32-position step
-  static constexpr int LOOP = STEP + 8 * 64;
+  static constexpr int LOW = STEP + 8 * 64;                // h16 [2 pairs of tiles][2][32 rows] of XS bytes: the folded low band
+  static constexpr int COEF = LOW + (BAND ? 4 * 32 * XS : 0);  // h16 [2 pairs of tiles][2][64 lanes][8]: what folds it
+  static constexpr int LOOP = COEF + (BAND ? 4096 : 0);
   static constexpr int STAT = 4 * 4 * 512 * 4;             // (epilogue, over the loop's) float slabs [4 waves][4 heads][512], then
   static constexpr int BYTES = LOOP > STAT + 160 ? LOOP : STAT + 160;   // statistics [4 waves][4 heads][2], sums [4], maxima [4]
 };
 
 // NKS: 16-column blocks of the (padded) key rank.  NC: 128-column chunks of the (padded) value rank.  NH: heads computed.
-template <int NKS, int NC, int NH>
+// BAND: the pairs 32 .. 63 as polynomials of the position (four heads only).
+template <int NKS, int NC, int NH, bool BAND>
 __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnParams p) {
-  using L = PaLds<NKS, NH>;
+  static_assert(!BAND || NH == 4, "a block of 32 rows is four heads of eight");
+  using L = PaLds<NKS, NH, BAND>;
   constexpr int TILE = PA_TILE;
   constexpr int NB = TILE / 32;                            // 32-position blocks
-  constexpr int MB = NH / 2;                               // matrix blocks of two heads
+  constexpr int MB = BAND ? 1 : NH / 2;                    // matrix blocks of 32 rows: two heads, or in the high band four
+  constexpr int ND = BAND ? 2 : 4;                         // RoPE pairs of a lane
   constexpr int KROWS = TILE / 8;                          // key rows of a tile that a score wave turns into fp16
   constexpr int KL = 64 / KROWS;                           // lanes of a key row
   constexpr int UL = 2 * NKS / KL;                         // words of codes of such a lane
@@ -182,7 +194,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
   float* const stat = reinterpret_cast<float*>(smem + L::STAT);
 
   // ---- this workgroup's piece of the line
-  int at = 0, end = 0;
+  int at = 0, end = 0, chunk = 1;
   int b = 0;
   int base = 0;                                            // where sequence b begins on the line
   if (p.direct) {
@@ -196,7 +208,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
     } else {
       total = pa_line(p, lane, -1).total;
     }
-    const int chunk = pa_chunk(p, total, gridDim.x);
+    chunk = pa_chunk(p, total, gridDim.x);
     const int64_t start = (int64_t)blockIdx.x * chunk;
     if (start >= total) return;                            // behind the line's end
     at = (int)start;
@@ -228,7 +240,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       ++b;
       continue;
     }
-    int gv, t0, t1;
+    int gv, t0, t1, last = 0;
     if (p.direct) {
       gv = blockIdx.x - b * GV;
       t0 = 0;
@@ -240,6 +252,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       t0 = max(into, 0);
       t1 = min(nt, into + (end - at));
       at += nt - into;                                     // where the next set begins
+      last = (at - 1) / chunk;                             // the piece that ends this one
       if (t1 <= t0) break;                                 // (the piece ends inside the fixed part: its tiles are the next piece's)
     }
     const int g = gv / p.VG, vg = gv - g * p.VG;
@@ -250,15 +263,13 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
 
     const int log_p = p.log_p, kw = p.Rk >> 3, vw = p.Rv >> 3;
     // Pages of 16 positions of a tile (never across a page's end), of 64 tiles at once: lane i has tile tb + i's, so that no tile waits
-    // for the table.  None: 0 (a page that exists; the rows are masked); outside the pool: -1.
-    auto load_pages = [&](int tb, int offset) {
-      const int64_t l = (int64_t)(tb + lane) * TILE + offset;
-      int pg = 0;
-      if (tb + lane < t1 && l < rows) {
-        pg = table[l >> log_p];
-        if (pg >= p.n_pages) pg = -1;
-      }
-      return pg;
+    // for the table.  Outside the pool: negative.
+    auto load_pages = [&](int tb, int offset) {            // (behind the rows: the last one's page again, those rows are masked)
+      return table[(int)min((int64_t)(tb + lane) * TILE + offset, (int64_t)rows - 1) >> log_p];
+    };
+    auto page_of = [&](int pages, int i) {
+      const int pg = __builtin_amdgcn_readlane(pages, i);
+      return pg < p.n_pages ? pg : -1;
     };
     auto slot_of = [&](int t, int offset, int pg) {        // first of those rows in the pool
       return (((int64_t)max(pg, 0) * p.G + g) << log_p) + ((t * TILE + offset) & ((1 << log_p) - 1));
@@ -270,6 +281,29 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
     const h16x2 m0 = {(h16)16384.f, (h16)16384.f}, m1 = {(h16)1024.f, (h16)1024.f};
     auto scaled = [&](unsigned bits, h16x2 mul, h16x2 z) { return __builtin_elementwise_fma(__builtin_bit_cast(h16x2, bits), mul, z); };
 
+    auto turn = [&](double a, float quarter, float& c, float& s) {        // v_sin / v_cos take revolutions: off by 1.2e-7 at most
+      const double rev = a * 0.15915494309189533577;
+      const float f = (float)(rev - rint(rev)) + quarter;
+      c = __builtin_amdgcn_cosf(f);
+      s = __builtin_amdgcn_sinf(f);
+    };
+    // Low band: what folds the 64 (pair, cos or sin) of tiles t0 + 2 u and the next into eight rows each.  Thread id of 512 has pair
+    // 32 + id / 16 (frequency f) and tile and term n = id % 8; k = 2^-5 (64 f)^n / n!.
+    auto low_factor = [&](float f, int n) {
+      float k = 0x1p-5f;
+#pragma unroll
+      for (int i = 1; i < 8; ++i) k *= i <= n ? 64.f / i * f : 1.f;
+      return k;
+    };
+    auto low_coefs = [&](int u, int id, float f, float k) {
+      pa_opaque(id);
+      const int col = id & 15, r = 2 * (id >> 4);
+      float c, s;
+      turn(((double)((t0 + 2 * u + (col >> 3)) * TILE + TILE / 2) - (double)qp) * (double)f, 0.25f * (col & 7), c, s);
+      *reinterpret_cast<h16x2*>(smem + L::COEF + (u & 1) * 2048 + (r >> 5) * 1024 + (((r >> 3) & 3) * 16 + col) * 16 + (r & 7) * 2) =
+          h16x2{(h16)(c * k), (h16)(s * k)};
+    };
+
     if (w < 8) {
       // ================================================ scores
       const int n = lane & 31, hi = lane >> 5;
@@ -280,7 +314,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           tb = t;
           pages = load_pages(t, KROWS * w);
         }
-        const int64_t slot = slot_of(t, KROWS * w, __builtin_amdgcn_readlane(pages, t - tb));
+        const int64_t slot = slot_of(t, KROWS * w, page_of(pages, t - tb));
         int ln = lane;
         pa_opaque(ln);
         const int krow = ln / KL, kpart = ln % KL;         // (a lane behind the row's end takes its last words: F is zero there)
@@ -301,32 +335,43 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       auto dequant_dst = [&](int buf, int ln) {
         return smem + buf * (TILE * L::XS) + (KROWS * w + ln / KL) * L::XS + ln % KL * UL * 16;
       };
-      load_k(t0);
 
       // ---- fold the query into B: row m of an A fragment is (head m / 16 of the block's two, column (pair, cos or sin)), a lane has 8
       // values of r.  The query is scaled to 16 .. 32 by a power of two, so that the fold's rounding to fp16 (2^-11 of each element: a
       // score is a sum of 128 Rk independent ones) meets no subnormals; the value waves take the factor back.
+      [[maybe_unused]] float lw = 0.f;
+      if constexpr (BAND) lw = p.inv_freq[32 + (tid >> 4)];
       h16x8 F[MB][NKS];
+      [[maybe_unused]] h16x8 FL[BAND ? NKS : 1];           // low band: [16 columns][32 of the 64 (pair, cos or sin)]
       {
-        const int e = n & 3, pair = 8 * w + 4 * ((n >> 3) & 1) + 2 * ((n >> 2) & 1) + (e >> 1);
-        const h16x8* frag = reinterpret_cast<const h16x8*>(p.bfrag) + ((int64_t)(gv * 8 + w) * MB * NKS) * 64 + lane;
+        // (row m, NH * 16 rows of pairs a wave: head m / 16 and pair 8 w + .., or head m / 8 and pair 4 w + ..)
+        const int e = n & 3, fh = BAND ? n >> 3 : n >> 4;
+        const int pair = 2 * ND * w + (BAND ? 0 : 4 * ((n >> 3) & 1)) + 2 * ((n >> 2) & 1) + (e >> 1);
+        const h16x8* frag = reinterpret_cast<const h16x8*>(p.bfrag) + (BAND ? p.band_at + (int64_t)(gv * 8 + w) * 2 * NKS * 64 :
+                                                                               (int64_t)(gv * 8 + w) * MB * NKS * 64) + lane;
         const h16* q = p.q + (int64_t)b * p.sq_b + (int64_t)h0 * p.sq_h;
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)                    // (all requests first; the fold is in place)
 #pragma unroll
           for (int kb = 0; kb < NKS; ++kb) F[mb][kb] = frag[(mb * NKS + kb) * 64];
+        if constexpr (BAND) {
+#pragma unroll
+          for (int i = 0; i < NKS; ++i) FL[i] = frag[(NKS + i) * 64];
+        }
         h16 qa[MB], qb[MB];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-          const h16* qr = q + min(2 * mb + (n >> 4), nh - 1) * p.sq_h + pair;
+          const h16* qr = q + min(2 * mb + fh, nh - 1) * p.sq_h + pair;
           qa[mb] = qr[0];
           qb[mb] = qr[64];
         }
         const int ex = pa_query_exponent(q, p.sq_h, nh, lane);
+        load_k(t0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-          const int e0 = __builtin_amdgcn_readlane(ex, 32 * mb), e1 = __builtin_amdgcn_readlane(ex, 32 * mb + 16);
-          const float f = __builtin_bit_cast(float, (unsigned)(127 - ((n >> 4) ? e1 : e0)) << 23);
+          const int ef = __builtin_amdgcn_ds_bpermute(64 * (2 * mb + fh), ex);          // (of lane 16 head)
+          const float f = __builtin_bit_cast(float, (unsigned)(127 - ef) << 23);
           const float q1 = (float)qa[mb] * f, q2 = (float)qb[mb] * f;
           const float own_f = (e & 1) ? -q1 : q1;
 #pragma unroll
@@ -342,34 +387,70 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
             pa_opaque(F[mb][kb]);                          // (done here: not, at the cost of twice the registers, at its use)
           }
         }
+        if constexpr (BAND) {                              // low band: a lane has both of B[r, i], B[r, i + 64] of four pairs a word
+          const int hl = w >> 1;
+          const h16* ql = q + min(hl, nh - 1) * p.sq_h + 32 + 4 * (lane >> 4);
+          const float f = __builtin_bit_cast(float, (unsigned)(127 - __builtin_amdgcn_readlane(ex, 16 * hl)) << 23);
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const h16x4 a = *reinterpret_cast<const h16x4*>(ql + 16 * ks), c = *reinterpret_cast<const h16x4*>(ql + 64 + 16 * ks);
+#pragma unroll
+            for (int rb = 0; rb < NKS / 2; ++rb) {
+              h16x8& x = FL[2 * rb + ks];
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                const float q1 = (float)a[d] * f, q2 = (float)c[d] * f, b1 = (float)x[2 * d], b2 = (float)x[2 * d + 1];
+                x[2 * d] = (h16)fmaf(b1, q1, b2 * q2);
+                x[2 * d + 1] = (h16)fmaf(b1, q2, -b2 * q1);
+              }
+              pa_opaque(x);
+            }
+          }
+        }
       }
 
-      // ---- rotation state: cos / sin of this lane's 4 pairs at position (block's first) + n, and (in LDS) of a step of 32
-      float tc[4], ts[4];
-      auto turn = [&](double a, float& c, float& s) {      // v_sin / v_cos take revolutions: off by 1.2e-7 at most
-        const double rev = a * 0.15915494309189533577;
-        const float f = (float)(rev - rint(rev));
-        c = __builtin_amdgcn_cosf(f);
-        s = __builtin_amdgcn_sinf(f);
+      // ---- low band: the rows that the coefficients fold F into (head w / 2, half the columns a wave), for two tiles at once
+      [[maybe_unused]] const float lk = low_factor(lw, tid & 7);
+      auto low_fold = [&](int u) {
+        int ln = lane;
+        pa_opaque(ln);
+        const char* const co = smem + L::COEF + (u & 1) * 2048 + ln * 16;
+        const h16x8 c0 = *reinterpret_cast<const h16x8*>(co), c1 = *reinterpret_cast<const h16x8*>(co + 1024);
+        const int col = ln & 15;
+        char* const to = smem + L::LOW + ((u & 1) * 2 + (col >> 3)) * 32 * L::XS + (8 * (w >> 1) + (col & 7)) * L::XS +
+                         (w & 1) * NKS * 16 + 8 * (ln >> 4);
+#pragma unroll
+        for (int rb = 0; rb < NKS / 2; ++rb) {
+          f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
+          d = __builtin_amdgcn_mfma_f32_16x16x32_f16(FL[2 * rb], c0, d, 0, 0, 0);
+          d = __builtin_amdgcn_mfma_f32_16x16x32_f16(FL[2 * rb + 1], c1, d, 0, 0, 0);
+          *reinterpret_cast<h16x4*>(to + 32 * rb) = h16x4{(h16)d[0], (h16)d[1], (h16)d[2], (h16)d[3]};
+        }
       };
+
+      // ---- rotation state: cos / sin of this lane's 4 pairs at position (block's first) + n, and (in LDS) of a step of 32
+      float tc[ND], ts[ND];
+      auto pair_of = [&](int d, int half) { return 2 * ND * w + (BAND ? 0 : 4 * (d >> 1)) + 2 * half + (d & 1); };
       auto start_angles = [&](int t) {
         int ln = lane;
         pa_opaque(ln);
-        const int at_n = (ln & 31) - qp;
-        const unsigned pair0 = 4 * (8 * w + 2 * (ln >> 5));
-        const double l = (double)(t * TILE + at_n);        // (below 2^30 + 2^30 in size)
+        const double l = (double)(t * TILE + (ln & 31)) - (double)qp;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const double wi = __builtin_bit_cast(float, lane_word(reinterpret_cast<const unsigned*>(p.inv_freq), pair0 + 16 * (i >> 1) + 4 * (i & 1)));
-          turn(l * wi, tc[i], ts[i]);
+        for (int i = 0; i < ND; ++i) {
+          const double wi = __builtin_bit_cast(float, lane_word(reinterpret_cast<const unsigned*>(p.inv_freq), 4 * pair_of(i, ln >> 5)));
+          turn(l * wi, 0.f, tc[i], ts[i]);
         }
       };
-      if (n < 4) {
+      if (n < ND) {
         float c, s;
-        turn(32.0 * (double)p.inv_freq[8 * w + 4 * (n >> 1) + 2 * hi + (n & 1)], c, s);
+        turn(32.0 * (double)p.inv_freq[pair_of(n, hi)], 0.f, c, s);
         float* o = reinterpret_cast<float*>(smem + L::STEP) + w * 16 + hi * 8 + n;
         o[0] = c;
         o[4] = s;
+      }
+      if constexpr (BAND) {
+        __syncthreads();                                   // (the value waves made the first coefficients)
+        low_fold(0);
       }
 #pragma unroll
       for (int i = 0; i < UL; ++i) dequant_word(dequant_dst(t0 & 1, lane), i);
@@ -394,7 +475,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         pa_opaque(ln);
         const char* const xt = smem + buf * (TILE * L::XS) + (ln & 31) * L::XS + (ln >> 5) * 16;
         char* const kdst = dequant_dst(buf ^ 1, ln);
-        float* const rdst = red + ((buf * 8 + w) * NH) * TILE + ln;
+        float* const rdst = red + ((buf * L::NP + w) * NH) * TILE + ln;
         const f32x4* const step = reinterpret_cast<const f32x4*>(smem + L::STEP) + w * 4 + (ln >> 5) * 2;
         constexpr int XD = 3;
         h16x8 x[XD];
@@ -402,6 +483,17 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         float part[2][NH];
         read_x(0);
         read_x(1);
+        // low band: positions 32 (w & 3) .., half of the columns
+        [[maybe_unused]] const int tr = t - t0;
+        [[maybe_unused]] const char *gl, *xl;
+        [[maybe_unused]] h16x8 gv8[2], xv8[2];
+        [[maybe_unused]] f32x16 yl = f32x16{};
+        if constexpr (BAND) {
+          gl = smem + L::LOW + (tr & 3) * 32 * L::XS + (ln & 31) * L::XS + (ln >> 5) * 16 + (w >> 2) * NKS * 16;
+          xl = xt + 32 * (w & 3) * L::XS + (w >> 2) * NKS * 16;
+          gv8[0] = *reinterpret_cast<const h16x8*>(gl);
+          xv8[0] = *reinterpret_cast<const h16x8*>(xl);
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           f32x16 y[MB];
@@ -413,12 +505,25 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
             if (i + 2 < NB * NKS) read_x(i + 2);
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb) y[mb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(F[mb][kb], x[i % XD], y[mb], 0, 0, 0);
+            if constexpr (BAND)
+              if (nb == 0 && kb < NKS / 2) {
+                yl = __builtin_amdgcn_mfma_f32_32x32x16_f16(gv8[kb & 1], xv8[kb & 1], yl, 0, 0, 0);
+                if (kb + 1 < NKS / 2) {
+                  gv8[(kb + 1) & 1] = *reinterpret_cast<const h16x8*>(gl + 32 * (kb + 1));
+                  xv8[(kb + 1) & 1] = *reinterpret_cast<const h16x8*>(xl + 32 * (kb + 1));
+                }
+              }
+            if constexpr (BAND)
+              if (nb == 2 && kb == 0) {                    // (a pair's rows were folded while the pair before was scored)
+                if (tr & 1) low_coefs(tr / 2 + 2, tid, lw, lk);
+                else low_fold(tr / 2 + 1);
+              }
             if (nb == 0 && kb < UL) dequant_word(kdst, kb);
             if (nb == (UL == NKS ? 1 : 0) && kb == (UL == NKS ? 0 : UL)) load_k(t + 2);   // (behind the range: page 0, not used)
             if (nb > 0 && kb == 0) {
               const f32x4 rc = step[0], rs = step[1];
 #pragma unroll
-              for (int d = 0; d < 4; ++d) {
+              for (int d = 0; d < ND; ++d) {
                 const float c = tc[d];
                 tc[d] = c * rc[d] - ts[d] * rs[d];
                 ts[d] = c * rs[d] + ts[d] * rc[d];
@@ -430,12 +535,30 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           for (int j = 0; j < NH; ++j) {
             float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              s0 = fmaf(y[j / 2][8 * (j & 1) + 2 * d], tc[d], s0);
-              s1 = fmaf(y[j / 2][8 * (j & 1) + 2 * d + 1], ts[d], s1);
+            for (int d = 0; d < ND; ++d) {
+              constexpr int JB = 16 / (2 * ND);            // heads of a block
+              s0 = fmaf(y[j / JB][2 * ND * (j % JB) + 2 * d], tc[d], s0);
+              s1 = fmaf(y[j / JB][2 * ND * (j % JB) + 2 * d + 1], ts[d], s1);
             }
             part[nb & 1][j] = s0 + s1;
           }
+          if constexpr (BAND)
+            if (nb == 0) {                                 // terms 4 hi .. 4 hi + 3 of four heads, in (position - 64) / 64
+              const float de = (float)((w & 3) * 32 + (ln & 31) - TILE / 2) * (2.f / TILE);
+              const float sc = ln & 32 ? 32.f * (de * de) * (de * de) : 32.f;
+              float low[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                low[j] = fmaf(fmaf(fmaf(yl[4 * j + 3], de, yl[4 * j + 2]), de, yl[4 * j + 1]), de, yl[4 * j]) * sc;
+              float* const ldst = red + ((buf * L::NP + 8 + (w >> 2)) * NH + (ln >> 5)) * TILE + 32 * (w & 3) + (ln & 31);
+#pragma unroll
+              for (int j = 0; j < 4; j += 2) {             // lanes 0 .. 31: head j, 32 .. 63: head j + 1
+                const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, low[j]), __builtin_bit_cast(unsigned, low[j + 1]),
+                                                                 false, false);
+                const unsigned lo = sw[0], up = sw[1];
+                ldst[j * TILE] = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, up);
+              }
+            }
           if (nb & 1) {
 #pragma unroll
             for (int j = 0; j < NH; ++j) {                 // the two halves of a position's columns; lane = position of the 64
@@ -449,7 +572,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         {                                                  // on to the next tile's first block
           const f32x4 rc = step[0], rs = step[1];
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
+          for (int d = 0; d < ND; ++d) {
             const float c = tc[d];
             tc[d] = c * rc[d] - ts[d] * rs[d];
             ts[d] = c * rs[d] + ts[d] * rc[d];
@@ -469,20 +592,20 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       unsigned vreg[NC][8], smk[2], smv[2];
       int tb = t0, pages0 = load_pages(t0, 32 * v), pages1 = load_pages(t0, 32 * v + 16);
       bool bad0, bad1;                                     // of the tile that is loaded
-      const unsigned* vsrc;                                // its values, this lane's first word
+      global_words vsrc;                                   // its values, this lane's first word
       auto next_tile = [&](int t) {                        // (behind the range: page 0 again, whose rows are masked)
         if (t - tb == 64) {
           tb = t;
           pages0 = load_pages(t, 32 * v);
           pages1 = load_pages(t, 32 * v + 16);
         }
-        const int pg0 = __builtin_amdgcn_readlane(pages0, t - tb), pg1 = __builtin_amdgcn_readlane(pages1, t - tb);
+        const int pg0 = page_of(pages0, t - tb), pg1 = page_of(pages1, t - tb);
         bad0 = pg0 < 0;
         bad1 = pg1 < 0;
         const int64_t slot0 = slot_of(t, 32 * v, pg0), slot1 = slot_of(t, 32 * v + 16, pg1);
         int ln = lane;
         pa_opaque(ln);
-        vsrc = p.vc + ((ln & 32 ? slot1 : slot0) + (ln & 16) / 2) * vw + (ln & 15);
+        vsrc = (global_words)p.vc + ((ln & 32 ? slot1 : slot0) + (ln & 16) / 2) * vw + (ln & 15);
         const unsigned pos4 = 4 * (ln & 15);
         smk[0] = lane_word(p.km + slot0, pos4);
         smk[1] = lane_word(p.km + slot1, pos4);
@@ -490,7 +613,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         smv[1] = lane_word(p.vm + slot1, pos4);
       };
       auto load_v = [&](int cc) {                          // (a column behind the row's end is read in front of it: never used)
-        const unsigned* src = vsrc + 16 * cc;
+        global_words src = vsrc + 16 * cc;
         if (cc == NC - 1) {
           int vcol = lane & 15;
           pa_opaque(vcol);
@@ -515,6 +638,16 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       for (int cc = 0; cc < NC; ++cc)
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[cc][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (BAND) {                                // the first two pairs of tiles' coefficients, while the others fold
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int id = tid - 512 + 256 * i;
+          const float f = p.inv_freq[32 + (id >> 4)], k = low_factor(f, id & 7);
+          low_coefs(0, id, f, k);
+          low_coefs(1, id, f, k);
+        }
+        __syncthreads();
+      }
       __syncthreads();
       __syncthreads();                                     // (the scores of the first tile)
 
@@ -522,16 +655,17 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         int ln = lane;
         pa_opaque(ln);
         const int head = ln >> 4, pos = ln & 15;
-        const float* const rt = red + ((t & 1) * 8 * NH + (NH == 4 ? head : head & (NH - 1))) * TILE + 32 * v + pos;
-        float part[2][8];
+        const float* const rt = red + ((t & 1) * L::NP * NH + (NH == 4 ? head : head & (NH - 1))) * TILE + 32 * v + pos;
+        float part[2][L::NP];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) part[h][k] = rt[k * NH * TILE + 16 * h];
+          for (int k = 0; k < L::NP; ++k) part[h][k] = rt[k * NH * TILE + 16 * h];
         float sc[2], sw[2], sv[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float s = ((part[h][0] + part[h][1]) + (part[h][2] + part[h][3])) + ((part[h][4] + part[h][5]) + (part[h][6] + part[h][7]));
+          if constexpr (BAND) s += part[h][8] + part[h][9];
           const h16x2 mk = __builtin_bit_cast(h16x2, smk[h]), mv = __builtin_bit_cast(h16x2, smv[h]);
           const bool valid = t * TILE + 32 * v + 16 * h + pos < rows && head < NH;
           s *= (float)mk[0] * hs;
@@ -645,15 +779,24 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
     const bool whole = t0 == 0 && t1 == nt;                // this workgroup has all of the sequence: the result itself
     const bool poison = pa_bad_len(p, b);
     const int64_t slot = (int64_t)blockIdx.x + b * GV + gv;      // (grows from piece to piece: a slot of its own for each)
-    for (int i = tid; i < nh * p.Rv; i += PA_THREADS) {
-      const int j = i / p.Rv, c = i - j * p.Rv;
-      const float* o = slab + j * 512 + c;
-      float v = 0.f;
+    {
+      const int j = tid / (PA_THREADS / 4), c = 4 * (tid % (PA_THREADS / 4));
+      if (j < nh && c < p.Rv) {
+        const float* o = slab + j * 512 + c;
+        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v += o[k * 2048];
-      if (whole) p.ctx[((int64_t)b * p.H + h0 + j) * p.Rv + c] = (h16)(poison ? NAN : v / stat[32 + j]);
-      else p.part[(int64_t)p.slots * 8 + (slot * 4 + j) * p.Rv + c] = v;
+        for (int k = 0; k < 4; ++k) v += *reinterpret_cast<const f32x4*>(o + k * 2048);
+        if (whole) {
+          const float f = poison ? NAN : 1.f / stat[32 + j];
+          *reinterpret_cast<h16x4*>(p.ctx + ((int64_t)b * p.H + h0 + j) * p.Rv + c) =
+              h16x4{(h16)(v[0] * f), (h16)(v[1] * f), (h16)(v[2] * f), (h16)(v[3] * f)};
+        } else {
+          *reinterpret_cast<f32x4*>(p.part + (int64_t)p.slots * 8 + (slot * 4 + j) * p.Rv + c) = v;
+        }
+      }
     }
+    static_assert(4 * (PA_THREADS / 4) >= 512, "columns of a head");
+    if (!p.direct && t0 == 0 && tid == 0) p.pieces[b * GV + gv] = {(int)blockIdx.x, last - (int)blockIdx.x + 1};
     if (!whole && tid < nh) {
       p.part[(slot * 4 + tid) * 2] = stat[36 + tid];
       p.part[(slot * 4 + tid) * 2 + 1] = stat[32 + tid];
@@ -673,10 +816,10 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
   }
 }
 
-template <int NKS, int NC, int NH>
+template <int NKS, int NC, int NH, bool BAND>
 int pa_launch1(const PagedAttnParams& p, int wgs, hipStream_t stream) {
-  auto kern = paged_attn_kernel<NKS, NC, NH>;
-  constexpr int lds = PaLds<NKS, NH>::BYTES;
+  auto kern = paged_attn_kernel<NKS, NC, NH, BAND>;
+  constexpr int lds = PaLds<NKS, NH, BAND>::BYTES;
   const int rc = palu_func_max_lds(reinterpret_cast<const void*>(kern), lds);
   if (rc != PALU_OK) return rc;
   hipLaunchKernelGGL(kern, dim3(wgs), dim3(PA_THREADS), lds, stream, p);
@@ -686,8 +829,8 @@ int pa_launch1(const PagedAttnParams& p, int wgs, hipStream_t stream) {
 template <int NKS, int NC>
 int pa_launch2(const PagedAttnParams& p, int heads, int wgs, hipStream_t stream) {
   if constexpr (NKS <= 8)
-    if (heads == 4) return pa_launch1<NKS, NC, 4>(p, wgs, stream);
-  return pa_launch1<NKS, NC, 2>(p, wgs, stream);
+    if (heads == 4) return p.band ? pa_launch1<NKS, NC, 4, true>(p, wgs, stream) : pa_launch1<NKS, NC, 4, false>(p, wgs, stream);
+  return pa_launch1<NKS, NC, 2, false>(p, wgs, stream);
 }
 template <int NKS>
 int pa_launch3(const PagedAttnParams& p, int chunks, int heads, int wgs, hipStream_t stream) {
