@@ -148,8 +148,10 @@ static __device__ __forceinline__ void lane_words(unsigned* out, const unsigned*
 }
 
 // Exponent of the largest element of head lane >> 4's query, less 4 (0 for a query of zeros, or one that is not finite).
-static __device__ __forceinline__ int pa_query_exponent(const h16* q, int64_t sq_h, int nh, int lane) {
-  const h16x8 q8 = *reinterpret_cast<const h16x8*>(q + min(lane >> 4, nh - 1) * sq_h + 8 * (lane & 15));
+static __device__ __forceinline__ h16x8 pa_query_part(const h16* q, int64_t sq_h, int nh, int lane) {
+  return *reinterpret_cast<const h16x8*>(q + min(lane >> 4, nh - 1) * sq_h + 8 * (lane & 15));
+}
+static __device__ __forceinline__ int pa_query_exponent(h16x8 q8) {
   float big = 0.f;
 #pragma unroll
   for (int d = 0; d < 8; ++d) big = fmaxf(big, fabsf((float)q8[d]));
@@ -234,7 +236,8 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
   }
 
   while (b < p.B) {
-    const int nt = __builtin_amdgcn_readfirstlane(pa_tiles(p, b));
+    const int len = __builtin_amdgcn_readfirstlane(p.lens[b]), room = p.max_pages << p.log_p;
+    const int rows = min(max(len, 0), room), nt = (rows + TILE - 1) / TILE;
     if (nt == 0) {
       if (p.direct) break;
       ++b;
@@ -257,7 +260,6 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
     }
     const int g = gv / p.VG, vg = gv - g * p.VG;
     const int h0 = g * p.gs + NH * vg, nh = min(NH, p.gs - NH * vg);
-    const int rows = __builtin_amdgcn_readfirstlane(pa_rows(p, b));
     const int qp = p.qpos ? p.qpos[b] : 0;
     const int* const table = p.table + (int64_t)b * p.st_b;
 
@@ -350,14 +352,8 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         const h16x8* frag = reinterpret_cast<const h16x8*>(p.bfrag) + (BAND ? p.band_at + (int64_t)(gv * 8 + w) * 2 * NKS * 64 :
                                                                                (int64_t)(gv * 8 + w) * MB * NKS * 64) + lane;
         const h16* q = p.q + (int64_t)b * p.sq_b + (int64_t)h0 * p.sq_h;
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb)                    // (all requests first; the fold is in place)
-#pragma unroll
-          for (int kb = 0; kb < NKS; ++kb) F[mb][kb] = frag[(mb * NKS + kb) * 64];
-        if constexpr (BAND) {
-#pragma unroll
-          for (int i = 0; i < NKS; ++i) FL[i] = frag[(NKS + i) * 64];
-        }
+        // (all requests first, in the order in which they are waited for; the fold is in place)
+        const h16x8 q8 = pa_query_part(q, p.sq_h, nh, lane);
         h16 qa[MB], qb[MB];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
@@ -365,7 +361,26 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           qa[mb] = qr[0];
           qb[mb] = qr[64];
         }
-        const int ex = pa_query_exponent(q, p.sq_h, nh, lane);
+        [[maybe_unused]] h16x4 la[2], lb[2];
+        if constexpr (BAND) {
+          const h16* ql = q + min(w >> 1, nh - 1) * p.sq_h + 32 + 4 * (lane >> 4);
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            la[ks] = *reinterpret_cast<const h16x4*>(ql + 16 * ks);
+            lb[ks] = *reinterpret_cast<const h16x4*>(ql + 64 + 16 * ks);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int kb = 0; kb < NKS; ++kb) F[mb][kb] = frag[(mb * NKS + kb) * 64];
+        if constexpr (BAND) {
+#pragma unroll
+          for (int i = 0; i < NKS; ++i) FL[i] = frag[(NKS + i) * 64];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const int ex = pa_query_exponent(q8);
         load_k(t0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -388,18 +403,15 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           }
         }
         if constexpr (BAND) {                              // low band: a lane has both of B[r, i], B[r, i + 64] of four pairs a word
-          const int hl = w >> 1;
-          const h16* ql = q + min(hl, nh - 1) * p.sq_h + 32 + 4 * (lane >> 4);
-          const float f = __builtin_bit_cast(float, (unsigned)(127 - __builtin_amdgcn_readlane(ex, 16 * hl)) << 23);
+          const float f = __builtin_bit_cast(float, (unsigned)(127 - __builtin_amdgcn_readlane(ex, 16 * (w >> 1))) << 23);
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
-            const h16x4 a = *reinterpret_cast<const h16x4*>(ql + 16 * ks), c = *reinterpret_cast<const h16x4*>(ql + 64 + 16 * ks);
 #pragma unroll
             for (int rb = 0; rb < NKS / 2; ++rb) {
               h16x8& x = FL[2 * rb + ks];
 #pragma unroll
               for (int d = 0; d < 4; ++d) {
-                const float q1 = (float)a[d] * f, q2 = (float)c[d] * f, b1 = (float)x[2 * d], b2 = (float)x[2 * d + 1];
+                const float q1 = (float)la[ks][d] * f, q2 = (float)lb[ks][d] * f, b1 = (float)x[2 * d], b2 = (float)x[2 * d + 1];
                 x[2 * d] = (h16)fmaf(b1, q1, b2 * q2);
                 x[2 * d + 1] = (h16)fmaf(b1, q2, -b2 * q1);
               }
@@ -591,6 +603,15 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       // the values; all of it is made anew in every tile, as in the scores.
       unsigned vreg[NC][8], smk[2], smv[2];
       int tb = t0, pages0 = load_pages(t0, 32 * v), pages1 = load_pages(t0, 32 * v + 16);
+      if constexpr (BAND) {                                // the first two pairs of tiles' coefficients, while the others fold
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int id = tid - 512 + 256 * i;
+          const float f = p.inv_freq[32 + (id >> 4)], k = low_factor(f, id & 7);
+          low_coefs(0, id, f, k);
+          low_coefs(1, id, f, k);
+        }
+      }
       bool bad0, bad1;                                     // of the tile that is loaded
       global_words vsrc;                                   // its values, this lane's first word
       auto next_tile = [&](int t) {                        // (behind the range: page 0 again, whose rows are masked)
@@ -630,7 +651,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
 #pragma unroll
       for (int cc = 0; cc < NC; ++cc) load_v(cc);
       // factor of a finished product of head lane >> 4 (2^10: the latents are held as (c - z) 2^-10)
-      const int ex = pa_query_exponent(p.q + (int64_t)b * p.sq_b + (int64_t)h0 * p.sq_h, p.sq_h, nh, lane);
+      const int ex = pa_query_exponent(pa_query_part(p.q + (int64_t)b * p.sq_b + (int64_t)h0 * p.sq_h, p.sq_h, nh, lane));
       const float hs = p.scale * __builtin_bit_cast(float, (unsigned)(ex + 137) << 23);
       float m = -INFINITY, lsum = 0.f;
       f32x4 acc[NC][8];                                    // [chunk][column of the lane's 8][head], times 2^-10 2^8; the same in all four vq
@@ -638,16 +659,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       for (int cc = 0; cc < NC; ++cc)
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[cc][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (BAND) {                                // the first two pairs of tiles' coefficients, while the others fold
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int id = tid - 512 + 256 * i;
-          const float f = p.inv_freq[32 + (id >> 4)], k = low_factor(f, id & 7);
-          low_coefs(0, id, f, k);
-          low_coefs(1, id, f, k);
-        }
-        __syncthreads();
-      }
+      if constexpr (BAND) __syncthreads();                 // (those coefficients)
       __syncthreads();
       __syncthreads();                                     // (the scores of the first tile)
 
@@ -763,24 +775,31 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         stat[32 + j] = sum;
         stat[36 + j] = top;
       }
+      // lanes eq write head eq (all four have the same)
+      const float f = pa_other(mine, 4 * v + eq);
 #pragma unroll
-      for (int jj = 0; jj < NH; ++jj) {                    // lanes vq = jj write head jj
-        const float f = lane_value(mine, 4 * v + jj);
+      for (int cc = 0; cc < NC; ++cc) {
+        float x[8];
 #pragma unroll
-        for (int cc = 0; cc < NC; ++cc)
-          if (eq == jj && 16 * cc + ecol < vw) {
-            float* d = slab + (v * 4 + jj) * 512 + 8 * (16 * cc + ecol);
-            *reinterpret_cast<f32x4*>(d) = f32x4{acc[cc][0][jj] * f, acc[cc][1][jj] * f, acc[cc][2][jj] * f, acc[cc][3][jj] * f};
-            *reinterpret_cast<f32x4*>(d + 4) = f32x4{acc[cc][4][jj] * f, acc[cc][5][jj] * f, acc[cc][6][jj] * f, acc[cc][7][jj] * f};
-          }
+        for (int c = 0; c < 8; ++c) {
+          const f32x4 y = acc[cc][c];
+          x[c] = (NH == 4 ? (eq & 2 ? (eq & 1 ? y[3] : y[2]) : (eq & 1 ? y[1] : y[0])) : (eq & 1 ? y[1] : y[0])) * f;
+        }
+        if (eq < NH && 16 * cc + ecol < vw) {
+          float* d = slab + (v * 4 + eq) * 512 + 8 * (16 * cc + ecol);
+          *reinterpret_cast<f32x4*>(d) = f32x4{x[0], x[1], x[2], x[3]};
+          *reinterpret_cast<f32x4*>(d + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        }
       }
       __syncthreads();
     }
     const bool whole = t0 == 0 && t1 == nt;                // this workgroup has all of the sequence: the result itself
-    const bool poison = pa_bad_len(p, b);
+    const bool poison = len > room;
+    int te = tid;
+    pa_opaque(te);
     const int64_t slot = (int64_t)blockIdx.x + b * GV + gv;      // (grows from piece to piece: a slot of its own for each)
     {
-      const int j = tid / (PA_THREADS / 4), c = 4 * (tid % (PA_THREADS / 4));
+      const int j = te / (PA_THREADS / 4), c = 4 * (te % (PA_THREADS / 4));
       if (j < nh && c < p.Rv) {
         const float* o = slab + j * 512 + c;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -796,10 +815,10 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       }
     }
     static_assert(4 * (PA_THREADS / 4) >= 512, "columns of a head");
-    if (!p.direct && t0 == 0 && tid == 0) p.pieces[b * GV + gv] = {(int)blockIdx.x, last - (int)blockIdx.x + 1};
-    if (!whole && tid < nh) {
-      p.part[(slot * 4 + tid) * 2] = stat[36 + tid];
-      p.part[(slot * 4 + tid) * 2 + 1] = stat[32 + tid];
+    if (!p.direct && t0 == 0 && te == 0) p.pieces[b * GV + gv] = {(int)blockIdx.x, last - (int)blockIdx.x + 1};
+    if (!whole && te < nh) {
+      p.part[(slot * 4 + te) * 2] = stat[36 + te];
+      p.part[(slot * 4 + te) * 2 + 1] = stat[32 + te];
     }
     if (p.direct || at >= end) break;
     if (gv == GV - 1) {
