@@ -159,13 +159,13 @@ static __device__ __forceinline__ int pa_query_exponent(h16x8 q8) {
   return big > 0.f && big < INFINITY ? (int)(__builtin_bit_cast(unsigned, big) >> 23) - 131 : 0;
 }
 
-template <int NKS, int NH, bool BAND>
+template <int NKS, int NC, int NH, bool BAND>
 struct PaLds {
   static constexpr int XS = NKS * 32 + 16;                 // bytes of a position's row: 16 more, so that 8 lanes reading 16 bytes of 8 rows meet 8 bank groups
   static constexpr int NP = BAND ? 10 : 8;                 // partial scores of a position: of eight waves, and two of the low band
   static constexpr int RED = 2 * PA_TILE * XS;             // float [2][NP][NH heads][PA_TILE]
-  static constexpr int WGT = RED + 2 * NP * NH * PA_TILE * 4;  // h16 [4 waves]: weights [4 heads][32], zeros [32]
-  static constexpr int STEP = WGT + 4 * 160 * 2;           // f32x4 [8 waves][2 halves][2]: cos / sin of a 32-position step
+  static constexpr int WGT = RED + 2 * NP * NH * PA_TILE * 4;  // h16 [4 waves]: weights [4 heads][32], zeros [32] (of two blocks of positions: 128 + 128, 64)
+  static constexpr int STEP = WGT + 4 * 160 * 2 * (NC == 4 ? 2 : 1);           // f32x4 [8 waves][2 halves][2]: cos / sin of a 32-position step
   static constexpr int LOW = STEP + 8 * 64;                // h16 [2 pairs of tiles][2][32 rows] of XS bytes: the folded low band
   static constexpr int COEF = LOW + (BAND ? 4 * 32 * XS : 0);  // h16 [2 pairs of tiles][2][64 lanes][8]: what folds it
   static constexpr int LOOP = COEF + (BAND ? 4096 : 0);
@@ -178,7 +178,7 @@ struct PaLds {
 template <int NKS, int NC, int NH, bool BAND>
 __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnParams p) {
   static_assert(!BAND || NH == 4, "a block of 32 rows is four heads of eight");
-  using L = PaLds<NKS, NH, BAND>;
+  using L = PaLds<NKS, NC, NH, BAND>;
   constexpr int TILE = PA_TILE;
   constexpr int NB = TILE / 32;                            // 32-position blocks
   constexpr int MB = BAND ? 1 : NH / 2;                    // matrix blocks of 32 rows: two heads, or in the high band four
@@ -596,13 +596,21 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       __syncthreads();                                     // (the statistics)
       __syncthreads();                                     // (the slabs)
     } else {
-      // ================================================ softmax and values: positions 32 v .. 32 v + 31 of a tile
-      const int v = w - 8;
-      h16* const wgt = reinterpret_cast<h16*>(smem + L::WGT) + v * 160;
-      // A lane is (head lane >> 4, positions lane & 15 and 16 more) in the softmax, and (rows 8 (lane >> 4) .., words (lane & 15) + 16 cc) in
+      // ================================================ softmax and values: 32 PB positions, NW chunks of columns
+      // A wave takes 32 positions and all columns, or (beyond 384 columns, whose sums and codes would fill the registers: values just
+      // requested were spilled, 10.8 us a tile at 128 / 512 in place of 4.1) 64 positions and half of the columns.
+      constexpr int PB = NC == 4 ? 2 : 1, NW = NC / PB;
+      const int v = w - 8, pv = v / PB, c0 = 16 * NW * (v % PB);             // (c0: this wave's first word of a row)
+      h16* const wgt = reinterpret_cast<h16*>(smem + L::WGT) + v * (160 * PB);
+      // A lane is (head lane >> 4, positions lane & 15 + 16 h) in the softmax, and (rows 8 (lane >> 4) .., words (lane & 15) + 16 cc) in
       // the values; all of it is made anew in every tile, as in the scores.
-      unsigned vreg[NC][8], smk[2], smv[2];
-      int tb = t0, pages0 = load_pages(t0, 32 * v), pages1 = load_pages(t0, 32 * v + 16);
+      unsigned vreg[PB][NW][8], smk[2 * PB], smv[2 * PB];
+      int tb = t0, pages[2 * PB];
+      auto all_pages = [&](int t) {
+#pragma unroll
+        for (int h = 0; h < 2 * PB; ++h) pages[h] = load_pages(t, 32 * PB * pv + 16 * h);
+      };
+      all_pages(t0);
       if constexpr (BAND) {                                // the first two pairs of tiles' coefficients, while the others fold
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -612,51 +620,55 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           low_coefs(1, id, f, k);
         }
       }
-      bool bad0, bad1;                                     // of the tile that is loaded
-      global_words vsrc;                                   // its values, this lane's first word
-      auto next_tile = [&](int t) {                        // (behind the range: page 0 again, whose rows are masked)
+      bool bad[2 * PB];                                    // of the tile that is loaded
+      global_words vsrc[PB];                               // its values, this lane's first word
+      auto next_tile = [&](int t) {                        // (behind the range: the last page again, whose rows are masked)
         if (t - tb == 64) {
           tb = t;
-          pages0 = load_pages(t, 32 * v);
-          pages1 = load_pages(t, 32 * v + 16);
+          all_pages(t);
         }
-        const int pg0 = page_of(pages0, t - tb), pg1 = page_of(pages1, t - tb);
-        bad0 = pg0 < 0;
-        bad1 = pg1 < 0;
-        const int64_t slot0 = slot_of(t, 32 * v, pg0), slot1 = slot_of(t, 32 * v + 16, pg1);
         int ln = lane;
         pa_opaque(ln);
-        vsrc = (global_words)p.vc + ((ln & 32 ? slot1 : slot0) + (ln & 16) / 2) * vw + (ln & 15);
-        const unsigned pos4 = 4 * (ln & 15);
-        smk[0] = lane_word(p.km + slot0, pos4);
-        smk[1] = lane_word(p.km + slot1, pos4);
-        smv[0] = lane_word(p.vm + slot0, pos4);
-        smv[1] = lane_word(p.vm + slot1, pos4);
+#pragma unroll
+        for (int pb = 0; pb < PB; ++pb) {
+          const int pg0 = page_of(pages[2 * pb], t - tb), pg1 = page_of(pages[2 * pb + 1], t - tb);
+          bad[2 * pb] = pg0 < 0;
+          bad[2 * pb + 1] = pg1 < 0;
+          const int64_t slot0 = slot_of(t, 32 * (PB * pv + pb), pg0), slot1 = slot_of(t, 32 * (PB * pv + pb) + 16, pg1);
+          vsrc[pb] = (global_words)p.vc + ((ln & 32 ? slot1 : slot0) + (ln & 16) / 2) * vw + (ln & 15);
+          const unsigned pos4 = 4 * (ln & 15);
+          smk[2 * pb] = lane_word(p.km + slot0, pos4);
+          smk[2 * pb + 1] = lane_word(p.km + slot1, pos4);
+          smv[2 * pb] = lane_word(p.vm + slot0, pos4);
+          smv[2 * pb + 1] = lane_word(p.vm + slot1, pos4);
+        }
       };
-      auto load_v = [&](int cc) {                          // (a column behind the row's end is read in front of it: never used)
-        global_words src = vsrc + 16 * cc;
-        if (cc == NC - 1) {
+      auto load_v = [&](int pb, int cc) {                  // (a column behind the row's end is read in front of it: never used)
+        global_words src = vsrc[pb] + c0 + 16 * cc;
+        if (cc == NW - 1) {
           int vcol = lane & 15;
           pa_opaque(vcol);
-          if (16 * cc + vcol >= vw) src = vsrc - vcol;
+          if (c0 + 16 * cc + vcol >= vw) src = vsrc[pb] - vcol;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          vreg[cc][i] = *src;
+          vreg[pb][cc][i] = *src;
           src += vw;
           asm volatile("" : "+v"(src));
         }
       };
       next_tile(t0);
 #pragma unroll
-      for (int cc = 0; cc < NC; ++cc) load_v(cc);
+      for (int pb = 0; pb < PB; ++pb)
+#pragma unroll
+        for (int cc = 0; cc < NW; ++cc) load_v(pb, cc);
       // factor of a finished product of head lane >> 4 (2^10: the latents are held as (c - z) 2^-10)
       const int ex = pa_query_exponent(pa_query_part(p.q + (int64_t)b * p.sq_b + (int64_t)h0 * p.sq_h, p.sq_h, nh, lane));
       const float hs = p.scale * __builtin_bit_cast(float, (unsigned)(ex + 137) << 23);
       float m = -INFINITY, lsum = 0.f;
-      f32x4 acc[NC][8];                                    // [chunk][column of the lane's 8][head], times 2^-10 2^8; the same in all four vq
+      f32x4 acc[NW][8];                                    // [chunk][column of the lane's 8][head], times 2^-10 2^8; the same in all four vq
 #pragma unroll
-      for (int cc = 0; cc < NC; ++cc)
+      for (int cc = 0; cc < NW; ++cc)
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[cc][c] = f32x4{0.f, 0.f, 0.f, 0.f};
       if constexpr (BAND) __syncthreads();                 // (those coefficients)
@@ -667,21 +679,21 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         int ln = lane;
         pa_opaque(ln);
         const int head = ln >> 4, pos = ln & 15;
-        const float* const rt = red + ((t & 1) * L::NP * NH + (NH == 4 ? head : head & (NH - 1))) * TILE + 32 * v + pos;
-        float part[2][L::NP];
+        const float* const rt = red + ((t & 1) * L::NP * NH + (NH == 4 ? head : head & (NH - 1))) * TILE + 32 * PB * pv + pos;
+        float part[2 * PB][L::NP];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2 * PB; ++h)
 #pragma unroll
           for (int k = 0; k < L::NP; ++k) part[h][k] = rt[k * NH * TILE + 16 * h];
-        float sc[2], sw[2], sv[2];
+        float sc[2 * PB], sw[2 * PB], sv[2 * PB];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2 * PB; ++h) {
           float s = ((part[h][0] + part[h][1]) + (part[h][2] + part[h][3])) + ((part[h][4] + part[h][5]) + (part[h][6] + part[h][7]));
           if constexpr (BAND) s += part[h][8] + part[h][9];
           const h16x2 mk = __builtin_bit_cast(h16x2, smk[h]), mv = __builtin_bit_cast(h16x2, smv[h]);
-          const bool valid = t * TILE + 32 * v + 16 * h + pos < rows && head < NH;
+          const bool valid = t * TILE + 32 * PB * pv + 16 * h + pos < rows && head < NH;
           s *= (float)mk[0] * hs;
-          if (h ? bad1 : bad0) s = NAN;
+          if (bad[h]) s = NAN;
           // The value's scale goes into the weight, and the maximum is that of s + log2 |scale|.  The weights' reference m follows it
           // only when it has grown by more than 2^7: weights then lie in 0 .. 2^15 and are held in fp16 to 2^-11 of themselves down
           // to 2^-22 of the largest, whatever the scales are, and the accumulators are hardly ever rescaled.  (The probabilities'
@@ -690,9 +702,11 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           const float sa = fabsf(sv[h]) < 0x1p-30f ? 0x1p-30f : fabsf(sv[h]);
           sc[h] = valid ? s : -INFINITY;
           sw[h] = sc[h] + __builtin_amdgcn_logf(sa);
-          if (ln < 16) wgt[128 + 16 * h + ln] = valid ? mv[1] * (h16)(-0.0009765625f) : (h16)0.f;
+          if (ln < 16) wgt[128 * PB + 16 * h + ln] = valid ? mv[1] * (h16)(-0.0009765625f) : (h16)0.f;
         }
-        const float top = row_max16(fmaxf(sw[0], sw[1]));
+        float most = fmaxf(sw[0], sw[1]);
+        if constexpr (PB == 2) most = fmaxf(most, fmaxf(sw[2], sw[3]));
+        const float top = row_max16(most);
         if (__ballot(top > m + 7.f)) {                     // (m is -inf at first: the first finite maximum is taken)
           const float mn = top > m + 7.f ? top : m;
           const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
@@ -702,49 +716,56 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           for (int j = 0; j < NH; ++j) {
             const float a = lane_value(alpha, 16 * j);
 #pragma unroll
-            for (int cc = 0; cc < NC; ++cc)
+            for (int cc = 0; cc < NW; ++cc)
 #pragma unroll
               for (int c = 0; c < 8; ++c) acc[cc][c][j] *= a;
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2 * PB; ++h) {
           const float we = __builtin_amdgcn_exp2f(sw[h] - (ref - 8.f));
-          wgt[head * 32 + 16 * h + pos] = (h16)(sv[h] == 0.f ? 0.f : __builtin_copysignf(we, sv[h]));
+          wgt[head * 32 + 128 * (h / 2) + 16 * (h % 2) + pos] = (h16)(sv[h] == 0.f ? 0.f : __builtin_copysignf(we, sv[h]));
           lsum += __builtin_amdgcn_exp2f(sc[h] - ref);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        const h16x8 a = *reinterpret_cast<const h16x8*>(wgt + (ln & 3) * 32 + 8 * head);
-        const u32x4 z4 = *reinterpret_cast<const u32x4*>(wgt + 128 + 8 * head);
+        h16x8 a[PB];
+        u32x4 z4[PB];
+#pragma unroll
+        for (int pb = 0; pb < PB; ++pb) {
+          a[pb] = *reinterpret_cast<const h16x8*>(wgt + 128 * pb + (ln & 3) * 32 + 8 * head);
+          z4[pb] = *reinterpret_cast<const u32x4*>(wgt + 128 * PB + 32 * pb + 8 * head);
+        }
         next_tile(t + 1);                                  // (its values are requested chunk by chunk, as the registers come free)
 #pragma unroll
-        for (int cc = 0; cc < NC; ++cc) {
+        for (int pb = 0; pb < PB; ++pb)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const unsigned sel = half ? 0x07060302u : 0x05040100u;
-            unsigned w0[4], w8[4];
+          for (int cc = 0; cc < NW; ++cc) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              w0[i] = __builtin_amdgcn_perm(vreg[cc][2 * i + 1], vreg[cc][2 * i], sel);
-              w8[i] = w0[i] >> 8;
+            for (int half = 0; half < 2; ++half) {
+              const unsigned sel = half ? 0x07060302u : 0x05040100u;
+              unsigned w0[4], w8[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                w0[i] = __builtin_amdgcn_perm(vreg[pb][cc][2 * i + 1], vreg[pb][cc][2 * i], sel);
+                w8[i] = w0[i] >> 8;
+              }
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                u32x4 x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  x[i] = __builtin_bit_cast(unsigned, scaled((c & 2 ? w8[i] : w0[i]) & (c & 1 ? 0x00F000F0u : 0x000F000Fu),
+                                                             c & 1 ? m1 : m0, __builtin_bit_cast(h16x2, (unsigned)z4[pb][i])));
+                acc[cc][4 * half + c] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(a[pb], __builtin_bit_cast(h16x8, x), acc[cc][4 * half + c], 0, 0, 0);
+              }
+              __builtin_amdgcn_sched_barrier(0);
             }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              u32x4 x;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                x[i] = __builtin_bit_cast(unsigned, scaled((c & 2 ? w8[i] : w0[i]) & (c & 1 ? 0x00F000F0u : 0x000F000Fu),
-                                                           c & 1 ? m1 : m0, __builtin_bit_cast(h16x2, (unsigned)z4[i])));
-              acc[cc][4 * half + c] =
-                  __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(h16x8, x), acc[cc][4 * half + c], 0, 0, 0);
-            }
+            load_v(pb, cc);
             __builtin_amdgcn_sched_barrier(0);
           }
-          load_v(cc);
-          __builtin_amdgcn_sched_barrier(0);
-        }
         __syncthreads();
       }
 
@@ -767,7 +788,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
 #pragma unroll
       for (int x = 4; x < 16; x <<= 1) top = fmaxf(top, pa_other(top, le ^ x));
       const float a = __builtin_amdgcn_exp2f(mk - (top == -INFINITY ? 0.f : top));
-      float sum = a * o[1];
+      float sum = k % PB ? 0.f : a * o[1];                 // (of the waves that share positions, one counts)
 #pragma unroll
       for (int x = 4; x < 16; x <<= 1) sum += pa_other(sum, le ^ x);
       const float mine = a * 4.f;                          // (2^10 2^-8)
@@ -778,15 +799,15 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       // lanes eq write head eq (all four have the same)
       const float f = pa_other(mine, 4 * v + eq);
 #pragma unroll
-      for (int cc = 0; cc < NC; ++cc) {
+      for (int cc = 0; cc < NW; ++cc) {
         float x[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           const f32x4 y = acc[cc][c];
           x[c] = (NH == 4 ? (eq & 2 ? (eq & 1 ? y[3] : y[2]) : (eq & 1 ? y[1] : y[0])) : (eq & 1 ? y[1] : y[0])) * f;
         }
-        if (eq < NH && 16 * cc + ecol < vw) {
-          float* d = slab + (v * 4 + eq) * 512 + 8 * (16 * cc + ecol);
+        if (eq < NH && c0 + 16 * cc + ecol < vw) {
+          float* d = slab + (pv * 4 + eq) * 512 + 8 * (c0 + 16 * cc + ecol);
           *reinterpret_cast<f32x4*>(d) = f32x4{x[0], x[1], x[2], x[3]};
           *reinterpret_cast<f32x4*>(d + 4) = f32x4{x[4], x[5], x[6], x[7]};
         }
@@ -804,7 +825,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         const float* o = slab + j * 512 + c;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v += *reinterpret_cast<const f32x4*>(o + k * 2048);
+        for (int k = 0; k < (NC == 4 ? 2 : 4); ++k) v += *reinterpret_cast<const f32x4*>(o + k * 2048);
         if (whole) {
           const float f = poison ? NAN : 1.f / stat[32 + j];
           *reinterpret_cast<h16x4*>(p.ctx + ((int64_t)b * p.H + h0 + j) * p.Rv + c) =
@@ -838,7 +859,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
 template <int NKS, int NC, int NH, bool BAND>
 int pa_launch1(const PagedAttnParams& p, int wgs, hipStream_t stream) {
   auto kern = paged_attn_kernel<NKS, NC, NH, BAND>;
-  constexpr int lds = PaLds<NKS, NH, BAND>::BYTES;
+  constexpr int lds = PaLds<NKS, NC, NH, BAND>::BYTES;
   const int rc = palu_func_max_lds(reinterpret_cast<const void*>(kern), lds);
   if (rc != PALU_OK) return rc;
   hipLaunchKernelGGL(kern, dim3(wgs), dim3(PA_THREADS), lds, stream, p);
