@@ -62,6 +62,8 @@ class PagePool(tuple):
         if any(r % 8 or r < 8 or r > 512 for r in (self.rank_k, self.rank_v)):
             raise ValueError(f"PagePool: group ranks must be multiples of 8 up to 512, got {self.rank_k}, {self.rank_v}")
         self._ptrs = tuple(t.data_ptr() for t in arrays)
+        self._sizes: dict = {}                                # (B, H, max_pages) -> bytes of the fragments and of the workspace
+        self._inv: dict = {}                                  # theta -> table of frequencies
         return self
 
     k_codes = property(lambda self: self[0])
@@ -97,12 +99,13 @@ def _pool(pool: PagePool, what: str, layers: bool = False) -> PagePool:
 
 
 def _launch(dev, fn, name: str, *args):
-    """fn(*args, stream) on the current stream of `dev`, which is made the current device if it is not"""
+    """fn(*args, stream) on the current stream of `dev`, which is made the current device if it is not.  (The stream's handle without
+    the Stream object around it: 2 us of a decode step's 12 us call.)"""
     if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, _lib.current_stream(dev))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _lib.current_stream(dev))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     if rc:
         _lib.check(rc, name)
 
@@ -110,9 +113,9 @@ def _launch(dev, fn, name: str, *args):
 def _int32(t: torch.Tensor, name: str, dim: int, dev, what: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim:
         raise TypeError(f"{what}: {name} must be an int32 tensor of {dim} dimension{'s' if dim > 1 else ''}")
-    if t.device != dev:
+    if t.get_device() != dev.index:
         raise ValueError(f"{what}: {name} must lie on {dev}, it is on {t.device}")
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
 
 
 def paged_append(pool: PagePool, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seq_ids: torch.Tensor,
@@ -147,7 +150,8 @@ def paged_append(pool: PagePool, k: torch.Tensor, v: torch.Tensor, block_table: 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """rows the kernels can load 16 bytes at a time"""
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    a, b, c = t.stride()
+    if c != 1 or a % 8 or b % 8 or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -237,13 +241,21 @@ def paged_attn(q: torch.Tensor, bfrag: torch.Tensor, pool: PagePool, block_table
     if table.shape[0] != B or lens.shape[0] != B or (qpos is not None and qpos.shape[0] != B):
         raise ValueError(f"{what}: block_table, seq_lens and q_positions must have one entry per query ({B})")
     lib = _lib.lib
-    need = lib.palu_paged_b_bytes(H, G, Rk)
+    sizes = pool._sizes.get((B, H, M))
+    if sizes is None:
+        if len(pool._sizes) > 1024:
+            pool._sizes.clear()
+        sizes = pool._sizes[B, H, M] = (lib.palu_paged_b_bytes(H, G, Rk),
+                                        lib.palu_paged_attn_workspace_bytes(B, H, G, M, P, Rk, Rv))
+    need = sizes[0]
     if need == 0 or bfrag.dtype != torch.uint8 or bfrag.numel() != need or bfrag.device != dev or not bfrag.is_contiguous():
         raise ValueError(f"{what}: bfrag is not prepare_paged_b's layout of a B for H={H}, num_groups={G}, Rk={Rk} on {dev}")
     q = _rows16(q)
     ctx = torch.empty((B, H, Rv), dtype=torch.float16, device=dev)
-    ws = torch.empty(lib.palu_paged_attn_workspace_bytes(B, H, G, M, P, Rk, Rv), dtype=torch.uint8, device=dev)
-    inv = rope_inv_freq(dev, D, theta)
+    ws = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
+    inv = pool._inv.get(theta)
+    if inv is None:
+        inv = pool._inv[theta] = rope_inv_freq(dev, D, theta)
     _launch(dev, lib.palu_paged_attn_q4, "palu_paged_attn_q4", q.data_ptr(), q.stride(0), q.stride(1), bfrag.data_ptr(), *pool._ptrs,
             table.data_ptr(), table.stride(0), M, lens.data_ptr(), 0 if qpos is None else qpos.data_ptr(), inv.data_ptr(),
             ctx.data_ptr(), ws.data_ptr(), B, H, G, D, P, pool.num_pages, Rk, Rv, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale))
