@@ -511,7 +511,10 @@ int palu_exchange_status(const void* buffer, unsigned* epoch_host, unsigned* err
  * position (the rotation is applied inside).  bfrag: palu_paged_prepare_b's layout of B [H][Rk][128] (made once, a weight).
  * ctx [B][H][Rv] contiguous.  A sequence of length 0 gives zeros; a length beyond max_pages * P or a page outside the pool within
  * the length gives NaN for that sequence (nothing outside the pool is read).  Rk <= 256, Rv <= 512.
- * The workspace may be reused once the call's work is done; two calls that run at the same time need one each.
+ * inv_freq [64] fp32.  A table that palu_rope_table_register knows, with 64 inv_freq[32] <= 0.7 rad, lets sets of four heads take the
+ * kernel's two-band form (about 1.2 times as fast at long lengths, the same to fp16 rounding).
+ * The workspace (written before it is read: it needs no clearing) may be reused once the call's work is done; two calls that run at the
+ * same time need one each.
  */
 int palu_paged_append_q4(const void* k, int64_t sk_t, int64_t sk_g, const void* v, int64_t sv_t, int64_t sv_g,
                          void* k_codes, void* k_meta, void* v_codes, void* v_meta,

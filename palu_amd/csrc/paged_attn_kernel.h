@@ -9,29 +9,47 @@
 //   score_l  = s_l sum_i cos((l - p) w_i) Yc_i + sin((l - p) w_i) Ys_i,     Y = F^T (c_l - z_l)
 // so no key is ever written down: Y is a matrix product (512 columns for four heads), the rotation a dot product in registers.
 //
+// Two bands (sets of four heads, 64 f_32 <= 0.7 rad): the pairs 32 .. 63 turn little within a tile of 128 positions.  With d =
+// (l - centre) / 64 in -1 .. 1 and a = (centre - p) w,
+//   cos((l - p) w) = sum_n (64 w)^n / n! cos(a + n pi / 2) d^n,       sin alike,
+// so the pairs' part of a score is sum_n d^n (G_n x) with G_n = sum_i (64 w_i)^n / n! (cos(a_i + n pi / 2) Fc_i + sin(..) Fs_i): eight
+// rows a head in place of 64, for one product [8 x 64] [64 x Rk] a head and tile (16 rows of v_mfma_f32_16x16x32_f16: two tiles at once).
+// n < 8 leaves 0.7^8 / 8! = 1.4e-6.  A tile costs 38 matrix blocks a wave instead of 64.
+//
 // Work: 2 Rk 512 + 2 Rv 4 flops a position and group of four heads against Rk / 2 + Rv / 2 + 8 bytes -- 500 flops a byte, so the
 // matrix pipe and the vector units bound it, not the memory.  Split:
 //   * A workgroup (12 waves, three a SIMD) takes a range of 128-position tiles of one (sequence, four heads of one latent group; two
 //     where Rk > 128, whose fragments fill the registers).  The work of the whole batch is one line, cut into
 //     gridDim.x equal pieces, so ragged batches need no plan from the host and replay in a graph; a piece that covers a sequence's end
 //     goes on with the next.  Pieces of one sequence are joined by a second kernel.
-//   * Scores: eight waves, wave w owns the RoPE pairs 8 w .. 8 w + 7 of all heads.  Its part of F stays in registers (4 heads x 16
-//     columns x Rk: 64 VGPRs at Rk = 128) as the A operand of v_mfma_f32_32x32x16_f16, two heads an instruction; a tile's codes are
-//     turned into fp16 once, by all eight waves, and shared through LDS as the B operand.  A lane then holds 4 pairs of ONE position
-//     for two heads, and the cos / sin of those 4 pairs, advanced from block to block by a rotation (exact again every 32 tiles),
-//     serve all heads.  The eight waves' partial scores meet in LDS.
+//   * Scores: eight waves, wave w owns the RoPE pairs 8 w .. 8 w + 7 of all heads (of the high band 4 w .. 4 w + 3).  Its part of F stays
+//     in registers (64 VGPRs at Rk = 128, with the low band's) as the A operand of v_mfma_f32_32x32x16_f16, two heads an instruction
+//     (four); a tile's codes are turned into fp16 once, by all eight waves, and shared through LDS as the B operand.  A lane then holds
+//     4 (2) pairs of ONE position for two (four) heads, and the cos / sin of those pairs, advanced from block to block by a rotation
+//     (exact again every 32 tiles), serve all heads.  The low band's product is dealt over the waves by position and column.  The
+//     partial scores meet in LDS.
 //   * Softmax and values: four waves, one a SIMD, each with 32 of a tile's positions and its own running maximum and sums, joined at
 //     the end of the range; they work on tile t - 1 while the others score tile t, so that the vector work of the values runs beside
 //     the matrix chains of the scores.  A lane holds eight columns of eight rows, as loaded, and so the B operands of eight
 //     v_mfma_f32_16x16x32_f16 (32 positions, 16 columns each; the four heads' weights fill its 16 rows four times over).  Smaller
 //     blocks (4x4x4, no idle row) were slower: every matrix instruction of a value wave waits for those of two score waves.
+//
+// Roundings to fp16, each by 2^-11 of the value at most: the folded query (low band: its coefficients and the folded rows too), whose
+// errors a score sums with random signs; the softmax weights; the result.  Sums, statistics, angles and rotations are 32 bits or more.
+// A whole is off by 4e-4 (ranks 64 / 192) to 7e-4 of its norm, of which the result's own rounding is 2e-4.  fp16 is what the matrix
+// unit takes at its full rate; F in two parts would cost twice the products.
+//
+// Measured: 3.1 us a tile and workgroup at ranks 128 / 384 in a short run (3.7 where the card's power limit holds the clock), 2.2 us at 64 / 192;
+// 10 to 12 us for a piece's start (launch, lengths, pages, 128 KB of B, the fold), first tile and end.  Half a million positions at 128 / 384:
+// 449 us, 1.22 PFLOP/s of the one-band form's work.  Matrix pipe busy 42 % of the cycles, vector units most of the rest: a tile takes 6.7 k
+// cycles, the score waves 4.2 to 5.6 k, the value waves 6.4 k, whichever of them have priority.
 #pragma once
 #include "palu_common.h"
 
 namespace {
 
 constexpr int PA_THREADS = 768;
-constexpr int PA_FIX = 3;                // cost of starting and ending a piece, in tiles (measured: 6 us against 2 us a tile)
+constexpr int PA_FIX = 3;                // cost of starting and ending a piece, in tiles (7 against 2.2 us, 12 against 3.1; 4 and 5: 1 to 5 % slower)
 constexpr int PA_TILE = 128;             // positions of a tile
 
 struct PagedAttnParams {

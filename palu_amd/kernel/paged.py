@@ -422,6 +422,8 @@ class PagedLatentCache:
         """Open a step that writes `tokens` new rows (one number, or one per sequence) to each of the distinct sequences `seqs`."""
         what = "begin"
         self._closed(what)
+        if self.pool.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedLatentCache.begin: not inside a graph capture (a replay would upload what the host held then)")
         ids = list(seqs)
         counts = [int(tokens)] * len(ids) if isinstance(tokens, Integral) else [int(t) for t in tokens]
         if not 1 <= len(ids) <= self.max_seqs or len(set(ids)) != len(ids):

@@ -287,3 +287,48 @@ def test_the_registered_ops_are_the_same_kernels():
     assert torch.equal(one, paged.paged_attn(q, frag, pool, moved, lens, lens - 1, THETA))
     with torch._subclasses.FakeTensorMode(allow_non_fake_inputs=True):
         assert torch.ops.palu.paged_attn(q, frag, *pool, table, lens).shape == (2, 8, 96)
+
+
+@torch.no_grad()
+def test_a_step_does_not_begin_inside_a_capture():
+    from palu_amd.kernel.palu_attention import PagedLatentCache
+    cache = PagedLatentCache(1, 2, 64, 64, num_pages=8, max_seqs=2, max_pages=4, page_size=16)
+    a = cache.add()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="not inside a graph capture"):
+            cache.begin([a])
+    cache.begin([a])
+    cache.abort()
+    assert cache.num_free == 7
+
+
+@torch.no_grad()
+def test_two_streams_work_on_two_caches_at_once():
+    """the same module, two caches, two streams: nothing of a call is shared but the weights"""
+    from palu_amd.kernel.palu_attention import PagedLatentCache
+    m = _module(0).prepare_decode(paged=True)
+    g = torch.Generator().manual_seed(5)
+    xs = [torch.randn((3, 1, 512), generator=g).half().cuda() for _ in range(2)]
+    prompts = [torch.randn((3, n, 512), generator=g).half().cuda() for n in (200, 333)]
+
+    def run(i):
+        cache = PagedLatentCache(1, 2, 64, 64, num_pages=80, max_seqs=3, max_pages=24, page_size=16)
+        ids = [cache.add() for _ in range(3)]
+        cache.begin(ids, tokens=prompts[i].shape[1])
+        m(prompts[i], past_key_value=cache, is_causal=True)
+        cache.commit()
+        outs = []
+        for _ in range(20):
+            cache.begin(ids)
+            outs.append(m(xs[i], past_key_value=cache)[0])
+            cache.commit()
+        return torch.cat(outs)
+    want = [run(0), run(1)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            got.append(run(i))
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
