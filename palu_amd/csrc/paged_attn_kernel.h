@@ -360,6 +360,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       // values of r.  The query is scaled to 16 .. 32 by a power of two, so that the fold's rounding to fp16 (2^-11 of each element: a
       // score is a sum of 128 Rk independent ones) meets no subnormals; the value waves take the factor back.
       [[maybe_unused]] float lw = 0.f;
+      [[maybe_unused]] float lk = 0.f;
       if constexpr (BAND) lw = p.inv_freq[32 + (tid >> 4)];
       h16x8 F[MB][NKS];
       [[maybe_unused]] h16x8 FL[BAND ? NKS : 1];           // low band: [16 columns][32 of the 64 (pair, cos or sin)]
@@ -398,6 +399,11 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           for (int i = 0; i < NKS; ++i) FL[i] = frag[(NKS + i) * 64];
         }
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (BAND) {                              // (while B is on its way)
+          lk = low_factor(lw, tid & 7);
+          low_coefs(0, tid, lw, lk);
+          low_coefs(1, tid, lw, lk);
+        }
         const int ex = pa_query_exponent(q8);
         load_k(t0);
         __builtin_amdgcn_sched_barrier(0);
@@ -440,7 +446,6 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       }
 
       // ---- low band: the rows that the coefficients fold F into (head w / 2, half the columns a wave), for two tiles at once
-      [[maybe_unused]] const float lk = low_factor(lw, tid & 7);
       auto low_fold = [&](int u) {
         int ln = lane;
         pa_opaque(ln);
@@ -479,7 +484,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         o[4] = s;
       }
       if constexpr (BAND) {
-        __syncthreads();                                   // (the value waves made the first coefficients)
+        __syncthreads();                                   // (the coefficients)
         low_fold(0);
       }
 #pragma unroll
@@ -629,15 +634,6 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         for (int h = 0; h < 2 * PB; ++h) pages[h] = load_pages(t, 32 * PB * pv + 16 * h);
       };
       all_pages(t0);
-      if constexpr (BAND) {                                // the first two pairs of tiles' coefficients, while the others fold
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int id = tid - 512 + 256 * i;
-          const float f = p.inv_freq[32 + (id >> 4)], k = low_factor(f, id & 7);
-          low_coefs(0, id, f, k);
-          low_coefs(1, id, f, k);
-        }
-      }
       bool bad[2 * PB];                                    // of the tile that is loaded
       global_words vsrc[PB];                               // its values, this lane's first word
       auto next_tile = [&](int t) {                        // (behind the range: the last page again, whose rows are masked)
@@ -689,7 +685,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       for (int cc = 0; cc < NW; ++cc)
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[cc][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (BAND) __syncthreads();                 // (those coefficients)
+      if constexpr (BAND) __syncthreads();                 // (the low band's first coefficients)
       __syncthreads();
       __syncthreads();                                     // (the scores of the first tile)
 
