@@ -186,9 +186,15 @@ struct PaLds {
   static constexpr int STEP = WGT + 4 * 160 * 2 * (NC == 4 ? 2 : 1);           // f32x4 [8 waves][2 halves][2]: cos / sin of a 32-position step
   static constexpr int LOW = STEP + 8 * 64;                // h16 [2 pairs of tiles][2][32 rows] of XS bytes: the folded low band
   static constexpr int COEF = LOW + (BAND ? 4 * 32 * XS : 0);  // h16 [2 pairs of tiles][2][64 lanes][8]: what folds it
-  static constexpr int LOOP = COEF + (BAND ? 4096 : 0);
-  static constexpr int STAT = 4 * 4 * 512 * 4;             // (epilogue, over the loop's) float slabs [4 waves][4 heads][512], then
-  static constexpr int BYTES = LOOP > STAT + 160 ? LOOP : STAT + 160;   // statistics [4 waves][4 heads][2], sums [4], maxima [4]
+  static constexpr int STAT = COEF + (BAND ? 4096 : 0);    // float: statistics [4 waves][4 heads][2], sums [4], maxima [4] of a finished piece
+  static constexpr int BYTES = STAT + 160;
+  // (a finished piece's sums, float slabs [4 waves][NH heads][512], lie over the partial scores)
+  static_assert(4 * NH * 512 * 4 <= WGT - RED, "room for the slabs");
+};
+
+template <bool SCORES>
+struct PaRole {
+  static constexpr bool value = SCORES;
 };
 
 // NKS: 16-column blocks of the (padded) key rank.  NC: 128-column chunks of the (padded) value rank.  NH: heads computed.
@@ -210,7 +216,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int GV = p.G * p.VG;
   float* const red = reinterpret_cast<float*>(smem + L::RED);
-  float* const slab = reinterpret_cast<float*>(smem);
+  float* const slab = red;
   float* const stat = reinterpret_cast<float*>(smem + L::STAT);
 
   // ---- this workgroup's piece of the line
@@ -253,29 +259,51 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
     end = __builtin_amdgcn_readfirstlane(end);
   }
 
-  while (b < p.B) {
-    const int len = __builtin_amdgcn_readfirstlane(p.lens[b]), room = p.max_pages << p.log_p;
-    const int rows = min(max(len, 0), room), nt = (rows + TILE - 1) / TILE;
-    if (nt == 0) {
-      if (p.direct) break;
-      ++b;
-      continue;
+  // Score waves and value waves go through the pieces each for themselves: the score waves fetch and fold the next piece's B while the
+  // value waves work off the last tile and join their sums.  Barriers of a piece of n tiles, in order: two in which the value waves join
+  // the piece before (at first: nothing), one after which the first tile's codes are there, one after each tile's scores.  Behind the
+  // last piece two more, for its own join.
+  int gv = 0, t0 = 0, t1 = 0, last = 0, len = 0, rows = 0, nt = 0;
+  const int room = p.max_pages << p.log_p;
+  auto find_piece = [&]() {
+    for (; b < p.B; ++b) {
+      len = __builtin_amdgcn_readfirstlane(p.lens[b]);
+      rows = min(max(len, 0), room);
+      nt = (rows + TILE - 1) / TILE;
+      if (nt > 0 || p.direct) break;
     }
-    int gv, t0, t1, last = 0;
+    if (b >= p.B || nt == 0) return false;
     if (p.direct) {
       gv = blockIdx.x - b * GV;
       t0 = 0;
       t1 = nt;
-    } else {
-      const int rel = at - base;                           // into sequence b
-      gv = rel / (nt + PA_FIX);
-      const int into = rel - gv * (nt + PA_FIX) - PA_FIX;  // tiles of this set of heads in front of `at` (negative: in its fixed part)
-      t0 = max(into, 0);
-      t1 = min(nt, into + (end - at));
-      at += nt - into;                                     // where the next set begins
-      last = (at - 1) / chunk;                             // the piece that ends this one
-      if (t1 <= t0) break;                                 // (the piece ends inside the fixed part: its tiles are the next piece's)
+      return true;
     }
+    const int rel = at - base;                             // into sequence b
+    gv = rel / (nt + PA_FIX);
+    const int into = rel - gv * (nt + PA_FIX) - PA_FIX;    // tiles of this set of heads in front of `at` (negative: in its fixed part)
+    t0 = max(into, 0);
+    t1 = min(nt, into + (end - at));
+    at += nt - into;                                       // where the next set begins
+    last = (at - 1) / chunk;                               // the piece that ends this one
+    return t1 > t0;                                        // (none: the piece ends inside the fixed part, its tiles are the next piece's)
+  };
+  auto next_piece = [&]() {
+    if (p.direct || at >= end) return false;
+    if (gv == GV - 1) {
+      base = at;
+      ++b;
+    }
+    return find_piece();
+  };
+  auto work = [&](auto role) {
+   constexpr bool SCORES = decltype(role)::value;
+   if (!find_piece()) return;
+   if constexpr (!SCORES) {
+     __syncthreads();
+     __syncthreads();
+   }
+   do {
     const int g = gv / p.VG, vg = gv - g * p.VG;
     const int h0 = g * p.gs + NH * vg, nh = min(NH, p.gs - NH * vg);
     const int qp = p.qpos ? p.qpos[b] : 0;
@@ -324,7 +352,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           h16x2{(h16)(c * k), (h16)(s * k)};
     };
 
-    if (w < 8) {
+    if constexpr (SCORES) {
       // ================================================ scores
       const int n = lane & 31, hi = lane >> 5;
       unsigned kreg[UL], kmeta;
@@ -483,10 +511,9 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         o[0] = c;
         o[4] = s;
       }
-      if constexpr (BAND) {
-        __syncthreads();                                   // (the coefficients)
-        low_fold(0);
-      }
+      __syncthreads();                                     // (the value waves' statistics of the piece before; this one's coefficients)
+      __syncthreads();                                     // (their slabs)
+      if constexpr (BAND) low_fold(0);
 #pragma unroll
       for (int i = 0; i < UL; ++i) dequant_word(dequant_dst(t0 & 1, lane), i);
       load_k(t0 + 1);
@@ -615,9 +642,6 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
         }
         __syncthreads();
       }
-      __syncthreads();                                     // (the values of the last tile)
-      __syncthreads();                                     // (the statistics)
-      __syncthreads();                                     // (the slabs)
     } else {
       // ================================================ softmax and values: 32 PB positions, NW chunks of columns
       // A wave takes 32 positions and all columns, or (beyond 384 columns, whose sums and codes would fill the registers: values just
@@ -685,11 +709,10 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       for (int cc = 0; cc < NW; ++cc)
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[cc][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (BAND) __syncthreads();                 // (the low band's first coefficients)
-      __syncthreads();
-      __syncthreads();                                     // (the scores of the first tile)
+      __syncthreads();                                     // (the first tile's codes)
 
       for (int t = t0; t < t1; ++t) {
+        __syncthreads();                                   // (its scores)
         int ln = lane;
         pa_opaque(ln);
         const int head = ln >> 4, pos = ln & 15;
@@ -780,7 +803,6 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
             load_v(pb, cc);
             __builtin_amdgcn_sched_barrier(0);
           }
-        __syncthreads();
       }
 
       // ---- join the four waves: the slabs of each through LDS, summed in a fixed order
@@ -821,47 +843,48 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
           x[c] = (NH == 4 ? (eq & 2 ? (eq & 1 ? y[3] : y[2]) : (eq & 1 ? y[1] : y[0])) : (eq & 1 ? y[1] : y[0])) * f;
         }
         if (eq < NH && c0 + 16 * cc + ecol < vw) {
-          float* d = slab + (pv * 4 + eq) * 512 + 8 * (c0 + 16 * cc + ecol);
+          float* d = slab + (pv * NH + eq) * 512 + 8 * (c0 + 16 * cc + ecol);
           *reinterpret_cast<f32x4*>(d) = f32x4{x[0], x[1], x[2], x[3]};
           *reinterpret_cast<f32x4*>(d + 4) = f32x4{x[4], x[5], x[6], x[7]};
         }
       }
       __syncthreads();
-    }
-    const bool whole = t0 == 0 && t1 == nt;                // this workgroup has all of the sequence: the result itself
-    const bool poison = len > room;
-    int te = tid;
-    pa_opaque(te);
-    const int64_t slot = (int64_t)blockIdx.x + b * GV + gv;      // (grows from piece to piece: a slot of its own for each)
-    {
-      const int j = te / (PA_THREADS / 4), c = 4 * (te % (PA_THREADS / 4));
-      if (j < nh && c < p.Rv) {
-        const float* o = slab + j * 512 + c;
-        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+      const bool whole = t0 == 0 && t1 == nt;              // this workgroup has all of the sequence: the result itself
+      const bool poison = len > room;
+      int te = tid - 512;
+      pa_opaque(te);
+      const int64_t slot = (int64_t)blockIdx.x + b * GV + gv;    // (grows from piece to piece: a slot of its own for each)
 #pragma unroll
-        for (int k = 0; k < (NC == 4 ? 2 : 4); ++k) v += *reinterpret_cast<const f32x4*>(o + k * 2048);
-        if (whole) {
-          const float f = poison ? NAN : 1.f / stat[32 + j];
-          *reinterpret_cast<h16x4*>(p.ctx + ((int64_t)b * p.H + h0 + j) * p.Rv + c) =
-              h16x4{(h16)(v[0] * f), (h16)(v[1] * f), (h16)(v[2] * f), (h16)(v[3] * f)};
-        } else {
-          *reinterpret_cast<f32x4*>(p.part + (int64_t)p.slots * 8 + (slot * 4 + j) * p.Rv + c) = v;
+      for (int i = 0; i < NH / 2; ++i) {
+        const int j = 2 * i + (te >> 7), c = 4 * (te & 127);
+        if (j < nh && c < p.Rv) {
+          const float* o = slab + j * 512 + c;
+          f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < (NC == 4 ? 2 : 4); ++k) v += *reinterpret_cast<const f32x4*>(o + k * (NH * 512));
+          if (whole) {
+            const float f = poison ? NAN : 1.f / stat[32 + j];
+            *reinterpret_cast<h16x4*>(p.ctx + ((int64_t)b * p.H + h0 + j) * p.Rv + c) =
+                h16x4{(h16)(v[0] * f), (h16)(v[1] * f), (h16)(v[2] * f), (h16)(v[3] * f)};
+          } else {
+            *reinterpret_cast<f32x4*>(p.part + (int64_t)p.slots * 8 + (slot * 4 + j) * p.Rv + c) = v;
+          }
         }
       }
+      if (!p.direct && t0 == 0 && te == 0) p.pieces[b * GV + gv] = {(int)blockIdx.x, last - (int)blockIdx.x + 1};
+      if (!whole && te < nh) {
+        p.part[(slot * 4 + te) * 2] = stat[36 + te];
+        p.part[(slot * 4 + te) * 2 + 1] = stat[32 + te];
+      }
     }
-    static_assert(4 * (PA_THREADS / 4) >= 512, "columns of a head");
-    if (!p.direct && t0 == 0 && te == 0) p.pieces[b * GV + gv] = {(int)blockIdx.x, last - (int)blockIdx.x + 1};
-    if (!whole && te < nh) {
-      p.part[(slot * 4 + te) * 2] = stat[36 + te];
-      p.part[(slot * 4 + te) * 2 + 1] = stat[32 + te];
-    }
-    if (p.direct || at >= end) break;
-    if (gv == GV - 1) {
-      base = at;
-      ++b;
-    }
-    __syncthreads();                                       // the slabs are read before the next piece's latents overwrite them
-  }
+   } while (next_piece());
+   if constexpr (SCORES) {
+     __syncthreads();
+     __syncthreads();
+   }
+  };
+  if (w < 8) work(PaRole<true>{});
+  else work(PaRole<false>{});
   if (p.direct && pa_tiles(p, b) == 0) {                   // an empty sequence: zeros
     const int gv = blockIdx.x % GV, g = gv / p.VG, vg = gv - g * p.VG;
     const int nh = min(NH, p.gs - NH * vg);
