@@ -647,6 +647,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       // A wave takes 32 positions and all columns, or (beyond 384 columns, whose sums and codes would fill the registers: values just
       // requested were spilled, 10.8 us a tile at 128 / 512 in place of 4.1) 64 positions and half of the columns.
       constexpr int PB = NC == 4 ? 2 : 1, NW = NC / PB;
+      __syncthreads();                                     // (the first tile's codes: the others go on while these fetch theirs)
       const int v = w - 8, pv = v / PB, c0 = 16 * NW * (v % PB);             // (c0: this wave's first word of a row)
       h16* const wgt = reinterpret_cast<h16*>(smem + L::WGT) + v * (160 * PB);
       // A lane is (head lane >> 4, positions lane & 15 + 16 h) in the softmax, and (rows 8 (lane >> 4) .., words (lane & 15) + 16 cc) in
@@ -709,8 +710,6 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
       for (int cc = 0; cc < NW; ++cc)
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[cc][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-      __syncthreads();                                     // (the first tile's codes)
-
       for (int t = t0; t < t1; ++t) {
         __syncthreads();                                   // (its scores)
         int ln = lane;
