@@ -36,20 +36,20 @@
 //
 // Roundings to fp16, each by 2^-11 of the value at most: the folded query (low band: its coefficients and the folded rows too), whose
 // errors a score sums with random signs; the softmax weights; the result.  Sums, statistics, angles and rotations are 32 bits or more.
-// A whole is off by 4e-4 (ranks 64 / 192) to 7e-4 of its norm, of which the result's own rounding is 2e-4.  fp16 is what the matrix
-// unit takes at its full rate; F in two parts would cost twice the products.
+// A result is off by 4e-4 to 1.1e-3 of its norm (one band: 7e-4), of which its own rounding is 2e-4.  fp16 is what the matrix unit takes
+// at its full rate; F in two parts would cost twice the products.
 //
-// Measured: 3.1 us a tile and workgroup at ranks 128 / 384 in a short run (3.7 where the card's power limit holds the clock), 2.2 us at 64 / 192;
-// 10 to 12 us for a piece's start (launch, lengths, pages, 128 KB of B, the fold), first tile and end.  Half a million positions at 128 / 384:
-// 449 us, 1.22 PFLOP/s of the one-band form's work.  Matrix pipe busy 42 % of the cycles, vector units most of the rest: a tile takes 6.7 k
-// cycles, the score waves 4.2 to 5.6 k, the value waves 6.4 k, whichever of them have priority.
+// Measured: 3.0 us a tile and workgroup at ranks 128 / 384 in a short run (3.7 where the card's power limit holds the clock), 2.1 us at
+// 64 / 192, beside 9 to 10 us for a launch, a piece's start (lengths, pages, 128 KB of B, the fold), first tile and end.  Half a million
+// positions at 128 / 384: 449 us, 1.22 PFLOP/s of the one-band form's work.  Matrix pipe busy 43 % of the cycles, vector units most of
+// the rest: a tile took 6.7 k cycles, the score waves 4.2 to 5.6 k of them, the value waves 6.4 k, whichever of them had priority.
 #pragma once
 #include "palu_common.h"
 
 namespace {
 
 constexpr int PA_THREADS = 768;
-constexpr int PA_FIX = 3;                // cost of starting and ending a piece, in tiles (7 against 2.2 us, 12 against 3.1; 4 and 5: 1 to 5 % slower)
+constexpr int PA_FIX = 3;                // cost of starting and ending a piece, in tiles (measured: 2 and 4: 1 to 5 % slower on ragged batches)
 constexpr int PA_TILE = 128;             // positions of a tile
 
 struct PagedAttnParams {
@@ -260,9 +260,9 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_kernel(PagedAttnPara
   }
 
   // Score waves and value waves go through the pieces each for themselves: the score waves fetch and fold the next piece's B while the
-  // value waves work off the last tile and join their sums.  Barriers of a piece of n tiles, in order: two in which the value waves join
-  // the piece before (at first: nothing), one after which the first tile's codes are there, one after each tile's scores.  Behind the
-  // last piece two more, for its own join.
+  // value waves work off the last tile and join their sums (16 sequences of 8 k: 59.4 us with all waves in step, 54.9 so).  Barriers of
+  // a piece of n tiles, in order: two in which the value waves join the piece before (at first: nothing), one when its result is out and
+  // the first tile's codes are there, one after each tile's scores.  Behind the last piece two more, for its own join.
   int gv = 0, t0 = 0, t1 = 0, last = 0, len = 0, rows = 0, nt = 0;
   const int room = p.max_pages << p.log_p;
   auto find_piece = [&]() {
