@@ -50,3 +50,61 @@ def test_long_sequences_cut_into_many_pieces(Rk, Rv):
     """pieces that begin at odd and even tiles, in the middle of a sequence and across the ends of several"""
     case = pages.Case([9000, 130, 0, 4097, 1, 2500, 128], G=3, Rk=Rk, Rv=Rv, P=64)
     case.check(pages._run(case))
+
+
+def test_more_sequences_than_the_plan_reads_at_once():
+    """a thousand sequences: every workgroup finds its piece in sixteen rounds of 64 lengths"""
+    case = pages.Case([(53 * i * i + 7 * i) % 290 if i % 5 else 0 for i in range(1000)], gs=1, G=1, Rk=32, Rv=32)
+    case.check(pages._run(case))
+
+
+def test_calls_with_nothing_in_them():
+    from palu_amd.kernel import paged
+    pool = paged.make_pool(2, 2, 16, 64, 96)
+    frag = paged.prepare_paged_b(torch.zeros(8, 64, 128).half().cuda(), 2)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    assert paged.paged_attn(torch.zeros(0, 8, 128).half().cuda(), frag, pool, torch.zeros(0, 3, **i32), torch.zeros(0, **i32)).shape == (0, 8, 96)
+    q = torch.ones(2, 8, 128).half().cuda()
+    out = paged.paged_attn(q, frag, pool, torch.zeros(2, 0, **i32), torch.tensor([0, 3], **i32))
+    assert bool((out[0] == 0).all()) and bool(out[1].isnan().all())          # a length that the table has no room for
+    before = [t.clone() for t in pool]
+    none = torch.zeros(0, **i32)
+    paged.paged_append(pool, torch.zeros(0, 2, 64).half().cuda(), torch.zeros(0, 2, 96).half().cuda(), torch.zeros(2, 1, **i32), none, none)
+    one = torch.zeros(1, **i32)
+    paged.paged_append(pool, torch.ones(1, 2, 64).half().cuda(), torch.ones(1, 2, 96).half().cuda(), torch.zeros(2, 0, **i32), one, one)
+    paged.paged_copy(pool, none, none)
+    paged.paged_copy(pool, [], [])
+    assert all(torch.equal(a, b) for a, b in zip(pool, before))
+
+
+@pytest.mark.parametrize("Rk,gs", [(64, 4), (64, 2), (192, 4)])
+def test_a_query_that_is_not_finite_spoils_its_head_only(Rk, gs):
+    case = pages.Case([200, 40], Rk=Rk, gs=gs)
+    good = pages._run(case)
+    case.q[0, 1, 5], case.q[1, 2, 100] = float("nan"), float("inf")
+    out = pages._run(case)
+    spoilt = torch.zeros(2, case.H, dtype=torch.bool)
+    spoilt[0, 1] = spoilt[1, 2] = True
+    assert bool(out[spoilt].isnan().all()) and torch.equal(out[~spoilt], good[~spoilt])
+
+
+def test_scores_of_another_scale():
+    from palu_amd.kernel import paged
+    case = pages.Case([300, 17])
+    same = paged.paged_attn(*case.args(), sm_scale=128 ** -0.5)
+    assert torch.equal(same, pages._run(case))
+    case.q *= 4                                                              # (a power of two: the same roundings)
+    assert torch.equal(paged.paged_attn(*case.args(), sm_scale=128 ** -0.5 / 4), same)
+
+
+def test_sequences_that_share_all_their_pages():
+    """the same rows under several table rows, one query each: what one sequence gives, for every one"""
+    from palu_amd.kernel import paged
+    case = pages.Case([700], Rk=128, Rv=384, P=64)
+    q, frag, pool, table, lens, pos = case.args()
+    qs = torch.cat([q, q * 0.5, q, q * 2])
+    many = paged.paged_attn(qs, frag, pool, table.expand(4, -1), lens.expand(4).contiguous(), pos.expand(4).contiguous())
+    ref, tol = case.reference()
+    for i in (0, 2):
+        assert bool(((many[i].double() - ref[0]).abs() <= tol[0]).all())
+    assert not torch.equal(many[1], many[0])
